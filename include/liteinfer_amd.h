@@ -168,6 +168,56 @@ int li_rope_kv_write_fp8(const void* q, const int64_t* q_strides, const void* k,
                          void* stream);
 
 /*
+ * Slot-write into an int8 cache with a scale for every (block, KV head), and
+ * its form with the rotary embedding. Layout: key_pool / value_pool
+ * [num_slots, num_kv_heads, head_dim] int8, key_scales / value_scales
+ * [num_slots / block_size, num_kv_heads] fp32 (rows scale_stride_block apart,
+ * heads adjacent), starting at zero; slot s of head h stands for
+ *     code * scale[s / block_size, h],   codes in -127 .. 127.
+ * Writing rows of one block and head, all in fp32:
+ *     old = 0 if the block's first slot is among them, else its scale
+ *     new = max(old, largest magnitude / 127, 2^-126)
+ *     the rows:       rint(x / new)           (as a product with 1 / new)
+ *     its other rows: rint(code * old / new)  (if new > old)
+ * A value that is not finite makes the scale NaN, until the block's first
+ * slot is written again. The entries of `slots` that name one block stand
+ * next to each other (a sequence's positions are consecutive and a block
+ * belongs to one sequence); the values stored are unspecified otherwise. A
+ * slot named twice keeps the later token; a slot outside the pool is skipped
+ * and counted into *bad_slots, as for li_kv_scatter. src_dtype / dtype:
+ * LI_F32, LI_F16 or LI_BF16.
+ *
+ * li_rope_kv_write_int8: q_out = q * cos + rotate_half(q) * sin rounded once
+ * to dtype, k rotated likewise and stored unrounded but for its code: fp32
+ * throughout, where li_rope_kv_write rounds each product as the separate
+ * torch ops do. Arguments as for li_rope_kv_write. No counterpart in the
+ * reference, whose roadmap (docs/roadmap.md, section 2.5) plans a quantised
+ * cache.
+ */
+#define LI_INT8_MAX_BLOCK 1024
+int li_kv_scatter_int8(const void* k, const void* v, const int64_t* k_strides,
+                       const int64_t* v_strides, int64_t batch, int64_t tokens,
+                       const int64_t* slots, void* key_pool, void* value_pool,
+                       float* key_scales, float* value_scales,
+                       int64_t num_slots, int block_size,
+                       int64_t pool_stride_slot, int64_t pool_stride_head,
+                       int64_t scale_stride_block, int num_kv_heads,
+                       int head_dim, int src_dtype, int32_t* bad_slots,
+                       void* stream);
+int li_rope_kv_write_int8(const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, const void* v,
+                          const int64_t* v_strides, const void* cos,
+                          const void* sin, const int64_t* cs_strides,
+                          int64_t batch, int64_t tokens, const int64_t* slots,
+                          void* q_out, const int64_t* q_out_strides,
+                          void* key_pool, void* value_pool, float* key_scales,
+                          float* value_scales, int64_t num_slots,
+                          int block_size, int64_t pool_stride_slot,
+                          int64_t pool_stride_head, int64_t scale_stride_block,
+                          int num_heads, int num_kv_heads, int head_dim,
+                          int dtype, int32_t* bad_slots, void* stream);
+
+/*
  * How many partitions each sequence's key loop is cut into for a decode step
  * of `batch` rows over a slot table `max_context` wide, on a device of
  * `num_cus` compute units (0 = ask the current device). The reference's

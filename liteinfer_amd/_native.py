@@ -45,6 +45,8 @@ EXPORTED_SYMBOLS = (
     "li_kv_scatter_fp8",
     "li_rope_kv_write",
     "li_rope_kv_write_fp8",
+    "li_kv_scatter_int8",
+    "li_rope_kv_write_int8",
     "li_choose_num_splits",
     "li_paged_decode_plan",
     "li_paged_decode",
@@ -99,6 +101,15 @@ _SIGNATURES = {
         _i32,
         [_p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i64p, _i64, _i64, _p, _p, _i64p, _p, _p,
          _i64, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _f32, _p, _p],
+    ),
+    "li_kv_scatter_int8": (
+        _i32,
+        [_p, _p, _i64p, _i64p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _p, _p],
+    ),
+    "li_rope_kv_write_int8": (
+        _i32,
+        [_p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i64p, _i64, _i64, _p, _p, _i64p, _p, _p, _p, _p,
+         _i64, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
     ),
     "li_choose_num_splits": (_i32, [_i32, _i32, _i32, _i32, _i32]),
     "li_paged_decode_plan": (
@@ -256,6 +267,14 @@ def check(status: int, what: str) -> None:
     if status in (LI_EINVAL, LI_EUNSUPPORTED, LI_EWORKSPACE):
         raise ValueError(message)
     raise RuntimeError(message)
+
+
+def on_device(device: torch.device, call, *args) -> int:
+    """`call(*args)` with `device` current: a launch goes to the current device, whatever stream it is given."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -52,6 +52,9 @@ class PagedKV(NamedTuple):
     """An fp8 (``torch.float8_e4m3fn``) pool holds K / k_scale; unused otherwise."""
     v_scale: float = 1.0
     """An fp8 pool holds V / v_scale; unused otherwise."""
+    key_scales: torch.Tensor | None = None
+    """``[num_blocks, kv_heads]`` float32: an int8 pool holds K over the scale of its block and head; None otherwise."""
+    value_scales: torch.Tensor | None = None
 
 
 # ---------------------------------------------------------------------------
@@ -73,12 +76,19 @@ def _causal_visibility(num_queries: int, num_keys: int, device: torch.device) ->
     return key_pos[None, :] <= query_pos[:, None]
 
 
-def _gather(pool: torch.Tensor, slots: torch.Tensor, like: torch.Tensor, scale: float) -> torch.Tensor:
+def _gather(pool: torch.Tensor, slots: torch.Tensor, like: torch.Tensor, scale: float,
+            block_scales: torch.Tensor | None = None) -> torch.Tensor:
     """``[B, W]`` slots of a ``[S, Hkv, D]`` pool -> ``[B, Hkv, W, D]`` in `like`'s dtype.
 
-    An fp8 pool's rows are dequantised (times `scale`) in float32, then
-    rounded to the query's dtype, the values the dense arithmetic then uses.
+    An fp8 pool's rows are dequantised (times `scale`) in float32, an int8
+    pool's times the scales of their blocks, then rounded to the query's
+    dtype, the values the dense arithmetic then uses.
     """
+    if pool.dtype == torch.int8:
+        if block_scales is None:
+            raise ValueError("an int8 pool needs key_scales and value_scales")
+        block = pool.shape[0] // block_scales.shape[0]
+        return (pool[slots] * block_scales[slots // block][..., None]).to(like.dtype).transpose(1, 2)
     rows = pool[slots].transpose(1, 2)
     if rows.dtype == torch.float8_e4m3fn:
         rows = (rows.to(torch.float32) * scale).to(like.dtype)
@@ -123,8 +133,8 @@ def _dense_decode(query: torch.Tensor, kv: PagedKV, attend: _Attend) -> torch.Te
     """Every row's context gathered at once, each bounded by its own length."""
     width = kv.slot_table.shape[1]
     bound = torch.arange(width, device=query.device)[None, :] < kv.context_lens.to(query.device)[:, None]
-    keys = _gather(kv.key_pool, kv.slot_table, query, kv.k_scale)
-    values = _gather(kv.value_pool, kv.slot_table, query, kv.v_scale)
+    keys = _gather(kv.key_pool, kv.slot_table, query, kv.k_scale, kv.key_scales)
+    values = _gather(kv.value_pool, kv.slot_table, query, kv.v_scale, kv.value_scales)
     return attend(query, keys, values, bound[:, None, None, :], False)
 
 
@@ -143,8 +153,8 @@ def _dense_packed(query: torch.Tensor, kv: PagedKV, attend: _Attend) -> torch.Te
         whole_prompt = nq == ctx
         is_causal = nq > 1 and whole_prompt
         visible = _causal_visibility(nq, ctx, query.device) if (nq > 1 and not whole_prompt) else None
-        keys = _gather(kv.key_pool, slots, chunk, kv.k_scale)
-        values = _gather(kv.value_pool, slots, chunk, kv.v_scale)
+        keys = _gather(kv.key_pool, slots, chunk, kv.k_scale, kv.key_scales)
+        values = _gather(kv.value_pool, slots, chunk, kv.v_scale, kv.value_scales)
         pieces.append(attend(chunk, keys, values, visible, is_causal))
     return torch.cat(pieces, dim=2)
 

@@ -28,7 +28,7 @@ class BlockPoolExhaustedError(RuntimeError):
     """The pool cannot hold what was asked of it."""
 
 
-CACHE_QUANT_FORMATS = (None, "fp8")
+CACHE_QUANT_FORMATS = (None, "fp8", "int8")
 
 
 class BlockPool:
@@ -38,7 +38,11 @@ class BlockPool:
     one byte per element: each row is written as ``x / k_scale`` (``v_scale``
     for V) rounded to e4m3 and read back times the scale — the reference's
     planned storage-level quantisation (docs/roadmap.md section 2.5, behind a
-    ``cache_quant`` flag). ``dtype`` stays the dtype K/V arrive and leave in.
+    ``cache_quant`` flag). ``cache_quant="int8"`` stores 8-bit integer codes
+    with a float32 scale for every (block, KV head), K and V apart, kept in
+    `block_scales` and grown as rows are appended (`paged_kernels.kv_scatter`):
+    no scale has to be known beforehand. ``dtype`` stays the dtype K/V arrive
+    and leave in.
     """
 
     def __init__(
@@ -67,13 +71,18 @@ class BlockPool:
         self.cache_quant = cache_quant
         self.k_scale = float(k_scale)
         self.v_scale = float(v_scale)
-        storage = torch.float8_e4m3fn if cache_quant == "fp8" else dtype
+        storage = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}.get(cache_quant, dtype)
         shape = (num_layers, num_blocks * block_size, num_kv_heads, head_dim)
         self._keys = torch.zeros(shape, dtype=storage, device=device)
         self._values = torch.zeros(shape, dtype=storage, device=device)
         # Every layer's view, made once: a layer's calls read them each step
         # (two index operations, ~1.5 us on the host, each time otherwise).
         self._layers = [(self._keys[i], self._values[i]) for i in range(num_layers)]
+        self._scales = None
+        self._layer_scales: list[tuple] = [(None, None)] * num_layers
+        if cache_quant == "int8":
+            self._scales = torch.zeros((2, num_layers, num_blocks, num_kv_heads), dtype=torch.float32, device=device)
+            self._layer_scales = [(self._scales[0, i], self._scales[1, i]) for i in range(num_layers)]
         self._free_blocks: list[int] = list(range(num_blocks))
         # Count of slot writes that named a slot outside the pool. The device
         # kernels skip such a write and add to this counter instead of raising.
@@ -81,8 +90,9 @@ class BlockPool:
 
     @property
     def nbytes(self) -> int:
-        """Device bytes held by keys and values together."""
-        return 2 * self._keys.numel() * self._keys.element_size()
+        """Device bytes held by keys and values together (an int8 pool's scales included)."""
+        scales = 0 if self._scales is None else self._scales.numel() * self._scales.element_size()
+        return 2 * self._keys.numel() * self._keys.element_size() + scales
 
     @property
     def device(self) -> torch.device:
@@ -122,6 +132,10 @@ class BlockPool:
     def slots(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         """This layer's flat key/value stores, ``[num_slots, num_kv_heads, head_dim]``."""
         return self._layers[layer_idx]
+
+    def block_scales(self, layer_idx: int) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+        """This layer's key / value scales, ``[num_blocks, num_kv_heads]``: an int8 pool's, else (None, None)."""
+        return self._layer_scales[layer_idx]
 
 
 _copy_streams: dict[int, torch.cuda.Stream] = {}

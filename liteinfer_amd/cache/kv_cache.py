@@ -47,21 +47,61 @@ def quantize_fp8(x: torch.Tensor, scale: float) -> torch.Tensor:
     return (x.to(torch.float32) * inv.to(x.device)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
 
 
+def append_int8(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor) -> None:
+    """Rows ``[tokens, heads, dim]`` into an int8 store at `slots`, in torch ops: what the HIP slot-write computes.
+
+    codes ``[num_slots, heads, dim]`` int8, scales ``[num_blocks, heads]``; all
+    arithmetic in float32 (`paged_kernels.kv_scatter` says what is stored). A
+    slot named twice keeps the later token.
+    """
+    block = codes.shape[0] // scales.shape[0]
+    named, place = torch.unique(slots, return_inverse=True)
+    last = torch.zeros_like(named).scatter_reduce_(0, place, torch.arange(slots.numel(), device=slots.device), "amax")
+    rows = rows.to(torch.float32)[last]
+    at, which = torch.unique(named // block, return_inverse=True)
+    held = scales[at]
+    old = held.index_fill(0, which[named % block == 0], 0.0)
+    largest = rows.abs().amax(dim=-1)
+    largest = torch.zeros_like(old).scatter_reduce_(0, which[:, None].expand_as(largest), largest, "amax")
+    new = torch.maximum(old, (largest * (1.0 / 127.0)).clamp(min=2.0 ** -126))
+    new = torch.where(torch.isfinite(new), new, float("nan"))
+    lost = torch.isnan(new)
+    inv = torch.where(lost, 0.0, 1.0 / new)
+    stored = codes.view(scales.shape[0], block, *codes.shape[1:])
+    before = stored[at]
+    again = torch.round(before * (old.nan_to_num() * inv)[:, None, :, None]).to(torch.int8)
+    stored[at] = torch.where((new > old)[:, None, :, None], again, before)
+    scales[at] = new
+    x = torch.where(lost[which][..., None], 0.0, rows * inv[which][..., None])
+    codes[named] = torch.round(x).clamp(-127, 127).to(torch.int8)
+
+
 def scatter_into(key_pool: torch.Tensor, value_pool: torch.Tensor, slots: torch.Tensor,
                  k: torch.Tensor, v: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0,
-                 bad_slots: torch.Tensor | None = None) -> None:
+                 bad_slots: torch.Tensor | None = None, key_scales: torch.Tensor | None = None,
+                 value_scales: torch.Tensor | None = None) -> None:
     """Store ``[B, H, T, D]`` K/V rows at `slots` (B*T entries, batch-major) of one layer's pools.
 
-    An fp8 pool stores each row quantised with its scale (`quantize_fp8`).
+    An fp8 pool stores each row quantised with its scale (`quantize_fp8`), an
+    int8 pool with the scales of its blocks (`append_int8`).
     On the device a slot outside the pool is skipped and counted into
     `bad_slots`; torch's indexed assignment raises for it on the CPU.
     """
     if key_pool.device.type == "cuda":
         from liteinfer_amd.paged_kernels import kv_scatter
 
-        kv_scatter(key_pool, value_pool, slots, k, v, k_scale=k_scale, v_scale=v_scale, bad_slots=bad_slots)
+        kv_scatter(key_pool, value_pool, slots, k, v, k_scale=k_scale, v_scale=v_scale, bad_slots=bad_slots,
+                   key_scales=key_scales, value_scales=value_scales)
         return
+    from liteinfer_amd.paged_kernels import check_block_scales
+
     flat = slots.reshape(-1)
+    if check_block_scales(key_pool, key_scales, value_scales):
+        if flat.numel() and not (0 <= int(flat.min()) and int(flat.max()) < key_pool.shape[0]):
+            raise IndexError(f"a slot is outside the pool's {key_pool.shape[0]}")
+        append_int8(key_pool, key_scales, flat, tokens_first(k))
+        append_int8(value_pool, value_scales, flat, tokens_first(v))
+        return
     if key_pool.dtype == torch.float8_e4m3fn:
         key_pool[flat] = quantize_fp8(tokens_first(k), k_scale)
         value_pool[flat] = quantize_fp8(tokens_first(v), v_scale)
@@ -150,7 +190,8 @@ class KVCache:
     def scatter(self, layer_idx: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Store one K/V column per slot, in the order the pass holds its tokens (kv_cache.py:236-247)."""
         keys, values = self._pool.slots(layer_idx)
-        scatter_into(keys, values, slots, k, v, self._pool.k_scale, self._pool.v_scale, self._pool.bad_slots)
+        scatter_into(keys, values, slots, k, v, self._pool.k_scale, self._pool.v_scale, self._pool.bad_slots,
+                     *self._pool.block_scales(layer_idx))
 
     def rotate_and_scatter(self, layer_idx: int, slots: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                            v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
@@ -160,14 +201,19 @@ class KVCache:
         of llama.py:85-98 and `scatter` on the CPU.
         """
         keys, values = self._pool.slots(layer_idx)
+        key_scales, value_scales = self._pool.block_scales(layer_idx)
         if keys.device.type == "cuda":
             from liteinfer_amd.rope import rope_kv_write
 
             return rope_kv_write(q, k, v, cos, sin, slots, keys, values,
                                  k_scale=self._pool.k_scale, v_scale=self._pool.v_scale,
-                                 bad_slots=self._pool.bad_slots)
+                                 bad_slots=self._pool.bad_slots, key_scales=key_scales, value_scales=value_scales)
         from liteinfer_amd.rope import apply_rotary_pos_emb
 
+        if key_scales is not None:  # float32 throughout, rounded once
+            q_embed, k_embed = apply_rotary_pos_emb(q.float(), k.float(), cos.float(), sin.float())
+            scatter_into(keys, values, slots, k_embed, v, key_scales=key_scales, value_scales=value_scales)
+            return q_embed.to(q.dtype)
         q_embed, k_embed = apply_rotary_pos_emb(q, k, cos, sin)
         scatter_into(keys, values, slots, k_embed, v, self._pool.k_scale, self._pool.v_scale)
         return q_embed
@@ -197,6 +243,7 @@ class _PackedPayload:
 
     def _paged_kv(self, layer_idx: int) -> PagedKV:
         key_pool, value_pool = self._cache.layer_storage(layer_idx)
+        key_scales, value_scales = self._cache.pool.block_scales(layer_idx)
         return PagedKV(
             key_pool,
             value_pool,
@@ -208,6 +255,8 @@ class _PackedPayload:
             host_query_lens=self._host_query_lens,
             k_scale=self._cache.pool.k_scale,
             v_scale=self._cache.pool.v_scale,
+            key_scales=key_scales,
+            value_scales=value_scales,
         )
 
 
@@ -236,5 +285,6 @@ class _DecodePayload:
     def _paged_kv(self, layer_idx: int) -> PagedKV:
         key_pool, value_pool = self._cache.layer_storage(layer_idx)
         pool = self._cache.pool
+        key_scales, value_scales = pool.block_scales(layer_idx)
         return PagedKV(key_pool, value_pool, self._slots, self._context_lens, self._num_splits,
-                       k_scale=pool.k_scale, v_scale=pool.v_scale)
+                       k_scale=pool.k_scale, v_scale=pool.v_scale, key_scales=key_scales, value_scales=value_scales)

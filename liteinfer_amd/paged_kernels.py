@@ -164,6 +164,36 @@ def _check_scales(k_scale: float, v_scale: float) -> None:
             raise ValueError(f"{name} must be finite and > 0, got {value}")
 
 
+def check_block_scales(key_pool: torch.Tensor, key_scales: torch.Tensor | None,
+                       value_scales: torch.Tensor | None) -> int:
+    """The block size of an int8 pool, from its scales: one for every (block of slots, KV head).
+
+    An int8 pool (``[num_slots, kv_heads, head_dim]`` codes) goes with
+    `key_scales` and `value_scales`, float32 ``[num_blocks, kv_heads]`` with
+    adjacent heads, where ``num_slots / num_blocks`` slots make a block. Other
+    pools take none: then the answer is 0.
+    """
+    if key_pool.dtype != torch.int8:
+        if key_scales is not None or value_scales is not None:
+            raise ValueError(f"block scales go with an int8 pool, not with {key_pool.dtype}")
+        return 0
+    if key_scales is None or value_scales is None:
+        raise ValueError("an int8 pool needs key_scales and value_scales")
+    num_slots, heads = key_pool.shape[:2]
+    for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != heads or (heads > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name} must be float32 [num_blocks, {heads}] with adjacent heads, "
+                             f"got {t.dtype} {list(t.shape)}")
+        if t.device != key_pool.device:
+            raise ValueError(f"{name} must be on {key_pool.device}, it is on {t.device}")
+    if key_scales.shape != value_scales.shape or key_scales.stride(0) != value_scales.stride(0):
+        raise ValueError("key and value scales must be laid out identically")
+    blocks = key_scales.shape[0]
+    if blocks == 0 or num_slots % blocks:
+        raise ValueError(f"{num_slots} slots are no whole number of slots for each of {blocks} blocks")
+    return num_slots // blocks
+
+
 def bad_slots_pointer(bad_slots: torch.Tensor | None, device: torch.device) -> int | None:
     """Device address of a slot-write miss counter (None for no counter)."""
     if bad_slots is None:
@@ -196,6 +226,8 @@ def kv_scatter(
     k_scale: float = 1.0,
     v_scale: float = 1.0,
     bad_slots: torch.Tensor | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
 ) -> None:
     """Store one K/V column per slot, in the order the pass holds its tokens.
 
@@ -206,6 +238,15 @@ def kv_scatter(
     for an fp8 (``torch.float8_e4m3fn``) pool, each element quantised as
     ``e4m3(clamp(x * (1 / scale), +-448))`` with ``k_scale`` / ``v_scale``
     (the reference's planned storage-level quantisation, roadmap section 2.5).
+
+    An int8 pool stores codes with a scale for every (block of slots, KV head)
+    in `key_scales` / `value_scales` (`check_block_scales`): a block's scale
+    grows to the largest magnitude appended to it over 127, and the rows it
+    held are re-expressed with it; writing a block's first slot starts it
+    anew. The slots of one block stand next to each other in `slots` (every
+    `KVCache` hands them out so); a slot named twice keeps the later token. A
+    value that is not finite turns its block's scale to NaN until the block is
+    started anew.
 
     A slot outside ``[0, num_slots)`` is not written. torch's ``index_put_``
     raises for it; a kernel cannot, so when `bad_slots` (a one-element int32
@@ -222,9 +263,10 @@ def kv_scatter(
     if heads != key_pool.shape[1] or head_dim != key_pool.shape[2]:
         raise ValueError(f"k rows {heads}x{head_dim} do not match the pool's {tuple(key_pool.shape[1:])}")
     fp8 = _is_fp8(key_pool)
-    if fp8:
+    block = check_block_scales(key_pool, key_scales, value_scales)
+    if fp8 or block:
         if k.dtype != v.dtype or k.dtype not in _native.DTYPE_CODES:
-            raise ValueError(f"an fp8 pool takes float32 / float16 / bfloat16 k and v, got {k.dtype}, {v.dtype}")
+            raise ValueError(f"an {'fp8' if fp8 else 'int8'} pool takes float32 / float16 / bfloat16 k and v, got {k.dtype}, {v.dtype}")
         _check_scales(k_scale, v_scale)
     elif k.dtype != key_pool.dtype or v.dtype != key_pool.dtype:
         raise ValueError(f"k/v dtype {k.dtype} does not match the pool's {key_pool.dtype}")
@@ -232,6 +274,18 @@ def kv_scatter(
     if flat_slots.numel() != batch * tokens:
         raise ValueError(f"{flat_slots.numel()} slots for {batch * tokens} tokens")
     lib = _native.load()
+    if block:
+        status = _native.on_device(
+            device, lib.li_kv_scatter_int8,
+            k.data_ptr(), v.data_ptr(),
+            _native.i64_array(k.stride()), _native.i64_array(v.stride()),
+            batch, tokens, flat_slots.data_ptr(),
+            key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+            key_pool.shape[0], block, key_pool.stride(0), key_pool.stride(1), max(key_scales.stride(0), heads),
+            heads, head_dim, _native.dtype_code(k.dtype), bad_ptr, _native.stream_handle(device),
+        )
+        _native.check(status, "kv_scatter")
+        return
     if fp8:
         status = lib.li_kv_scatter_fp8(
             k.data_ptr(), v.data_ptr(),

@@ -15,7 +15,8 @@ from __future__ import annotations
 import torch
 
 from liteinfer_amd import _native
-from liteinfer_amd.paged_kernels import _as_index, _check_pools, _require_device_tensors, bad_slots_pointer
+from liteinfer_amd.paged_kernels import (_as_index, _check_pools, _require_device_tensors, bad_slots_pointer,
+                                         check_block_scales)
 
 
 def rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -45,6 +46,8 @@ def rope_kv_write(
     k_scale: float = 1.0,
     v_scale: float = 1.0,
     bad_slots: torch.Tensor | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Rotate q and k, store k and v at `slots`, return the rotated q.
 
@@ -61,15 +64,21 @@ def rope_kv_write(
             (``torch.float8_e4m3fn``) pool stores the rotated k (rounded to
             q's dtype, as the torch ops round it) and v quantised with
             `k_scale` / `v_scale`, exactly as `kv_scatter` would store them.
+            An int8 pool stores the rotated k and v as codes with the scales
+            of their blocks (`kv_scatter`); q and k are then rotated in
+            float32 and rounded once, q to its dtype and k to its code, where
+            the other pools round every product as the torch ops do.
         bad_slots: optional one-element int32 counter of slots outside the
             pool (not written), as for `kv_scatter`.
+        key_scales, value_scales: an int8 pool's scales, ``[num_blocks,
+            num_kv_heads]`` float32, written in place with it.
 
     Returns:
         The rotated q, ``[batch, num_heads, tokens, head_dim]``, laid out
         token-major in memory like the reference's result (so the packed
         attention's ``squeeze(0).transpose(0, 1)`` is a free view).
     """
-    if q.is_cuda:
+    if q.is_cuda and key_scales is None:
         # Operands that need no conversion: checked and passed on in C++.
         out = _native.fast_calls().rope(q, k, v, cos, sin, slots, key_pool, value_pool, k_scale, v_scale, bad_slots,
                                         _native.stream_handle(q.device))
@@ -92,7 +101,10 @@ def rope_kv_write(
     if head_dim % 2:
         raise ValueError(f"head_dim {head_dim} must be even for rotary embedding")
     fp8 = key_pool.dtype == _native.FP8_POOL_DTYPE
-    dtype = q.dtype if fp8 else key_pool.dtype
+    block = check_block_scales(key_pool, key_scales, value_scales)
+    dtype = q.dtype if fp8 or block else key_pool.dtype
+    if block and dtype not in _native.DTYPE_CODES:
+        raise ValueError(f"an int8 pool is written from float32, float16 or bfloat16 projections, not {dtype}")
     if fp8 and dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"an fp8 pool is written from bfloat16 or float16 projections, not {dtype}")
     for name, t in (("q", q), ("k", k), ("v", v), ("cos", cos), ("sin", sin)):
@@ -111,6 +123,21 @@ def rope_kv_write(
         raise ValueError(f"{flat_slots.numel()} slots for {batch * tokens} tokens")
     out = torch.empty(batch, tokens, num_heads, head_dim, dtype=dtype, device=device).transpose(1, 2)
     lib = _native.load()
+    if block:
+        status = _native.on_device(
+            device, lib.li_rope_kv_write_int8,
+            q.data_ptr(), _native.i64_array(q.stride()),
+            k.data_ptr(), _native.i64_array(k.stride()),
+            v.data_ptr(), _native.i64_array(v.stride()),
+            cos.data_ptr(), sin.data_ptr(), _native.i64_array(cs_strides),
+            batch, tokens, flat_slots.data_ptr(),
+            out.data_ptr(), _native.i64_array(out.stride()),
+            key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+            key_pool.shape[0], block, key_pool.stride(0), key_pool.stride(1),
+            max(key_scales.stride(0), num_kv_heads), num_heads, num_kv_heads, head_dim, _native.dtype_code(dtype),
+            bad_ptr, _native.stream_handle(device))
+        _native.check(status, "rope_kv_write")
+        return out
     args = (
         q.data_ptr(), _native.i64_array(q.stride()),
         k.data_ptr(), _native.i64_array(k.stride()),
