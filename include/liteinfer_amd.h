@@ -443,6 +443,54 @@ int li_paged_prefill_ex(const void* q, int64_t q_stride_tok, int64_t q_stride_he
                         float k_scale, float v_scale, int flags, void* stream);
 
 /*
+ * li_paged_decode and li_paged_prefill over an int8 pool with a scale for
+ * every (block, KV head), as li_kv_scatter_int8 writes it: the same attention
+ * over code * scale. key_scales, value_scales, block_size and
+ * scale_stride_block as there; pool strides in codes (bytes). Queries of
+ * LI_F32, LI_F16 or LI_BF16, any head_dim up to 512 and any grouping. The
+ * decode's workspace is what li_paged_decode_plan reports. The packed pass
+ * needs what li_paged_prefill_int8_plan reports: it lays the chunks'
+ * contexts out in `dtype` once (each value rounded to it), which the pass's
+ * query blocks then share; context_tokens, the same in both calls, is the sum
+ * of context_lens where the caller knows it (0: batch x max_context), and a
+ * sum below the truth leaves the rows past it unspecified. No counterpart in
+ * the reference, whose roadmap (docs/roadmap.md, section 2.5) plans a
+ * quantised cache.
+ */
+int li_paged_decode_int8(const void* q, int64_t q_stride_seq,
+                         int64_t q_stride_head, const void* key_pool,
+                         const void* value_pool, const float* key_scales,
+                         const float* value_scales, int block_size,
+                         int64_t scale_stride_block, int64_t pool_stride_slot,
+                         int64_t pool_stride_head, const int64_t* slot_table,
+                         int64_t slot_table_stride, int max_context,
+                         const int32_t* context_lens, void* out,
+                         int64_t out_stride_seq, int64_t out_stride_head,
+                         int batch, int num_heads, int num_kv_heads,
+                         int head_dim, float scale, int num_splits,
+                         int block_kv, void* workspace, size_t workspace_bytes,
+                         int dtype, int flags, void* stream);
+int li_paged_prefill_int8_plan(int batch, int num_heads, int num_kv_heads,
+                               int head_dim, int max_context,
+                               int max_query_len, int64_t context_tokens,
+                               int dtype, size_t* workspace_bytes);
+int li_paged_prefill_int8(const void* q, int64_t q_stride_tok,
+                          int64_t q_stride_head, const void* key_pool,
+                          const void* value_pool, const float* key_scales,
+                          const float* value_scales, int block_size,
+                          int64_t scale_stride_block, int64_t pool_stride_slot,
+                          int64_t pool_stride_head, const int64_t* slot_table,
+                          int64_t slot_table_stride, int max_context,
+                          const int32_t* context_lens,
+                          const int32_t* query_start_loc, int batch,
+                          int max_query_len, int64_t context_tokens, void* out,
+                          int64_t out_stride_tok, int64_t out_stride_head,
+                          int num_heads, int num_kv_heads, int head_dim,
+                          float scale, int block_q, int block_kv,
+                          void* workspace, size_t workspace_bytes, int dtype,
+                          int flags, void* stream);
+
+/*
  * The minimal engine's per-layer elementwise work (the model around the
  * paged path; no counterpart in the reference's paged path, which leaves it
  * to torch ops). Rows of `hidden` (a multiple of 8, at most 8192) bf16 / fp16

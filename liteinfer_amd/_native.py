@@ -57,6 +57,9 @@ EXPORTED_SYMBOLS = (
     "li_prefill_row_groups",
     "li_paged_prefill",
     "li_paged_prefill_ex",
+    "li_paged_decode_int8",
+    "li_paged_prefill_int8_plan",
+    "li_paged_prefill_int8",
     "li_add_rms_norm",
     "li_silu_mul",
     "li_skinny_gemm_plan",
@@ -150,6 +153,17 @@ _SIGNATURES = {
         _i32,
         [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _p, _i64, _i64,
          _i32, _i32, _i32, _f32, _i32, _i32, _p, _sz, _i32, _i32, _f32, _f32, _i32, _p],
+    ),
+    "li_paged_decode_int8": (
+        _i32,
+        [_p, _i64, _i64, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _i64, _i64,
+         _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p, _sz, _i32, _i32, _p],
+    ),
+    "li_paged_prefill_int8_plan": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i64, _i32, ctypes.POINTER(_sz)]),
+    "li_paged_prefill_int8": (
+        _i32,
+        [_p, _i64, _i64, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _p, _p, _i32, _i32, _i64, _p, _i64, _i64,
+         _i32, _i32, _i32, _f32, _i32, _i32, _p, _sz, _i32, _i32, _p],
     ),
 }
 

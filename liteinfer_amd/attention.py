@@ -190,6 +190,7 @@ def _paged_decode_step(query: torch.Tensor, kv: PagedKV, scaling: float, num_kv_
     out = paged_decode(
         query.squeeze(2), kv.key_pool, kv.value_pool, kv.slot_table, kv.context_lens,
         scaling, num_kv_groups, num_splits=kv.num_splits, k_scale=kv.k_scale, v_scale=kv.v_scale,
+        key_scales=kv.key_scales, value_scales=kv.value_scales,
     )
     return out.unsqueeze(2)
 
@@ -231,7 +232,8 @@ def _paged_packed(query: torch.Tensor, kv: PagedKV, scaling: float, num_kv_group
     out = paged_prefill(
         query.squeeze(0).transpose(0, 1), kv.key_pool, kv.value_pool, kv.slot_table, kv.context_lens,
         kv.query_start_loc, kv.max_query_len, scaling, num_kv_groups, one_query_rows=one_query_rows,
-        k_scale=kv.k_scale, v_scale=kv.v_scale,
+        k_scale=kv.k_scale, v_scale=kv.v_scale, key_scales=kv.key_scales, value_scales=kv.value_scales,
+        context_tokens=sum(kv.host_context_lens) if kv.key_scales is not None and kv.host_context_lens else None,
     )
     return out.transpose(0, 1).unsqueeze(0)
 

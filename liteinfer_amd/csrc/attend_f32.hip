@@ -436,7 +436,7 @@ bool attend_f32_applies(const AttnArgs& a, int dtype) {
   // (A packed pass's grid is capped.)
   const int64_t units = (int64_t)a.batch * a.num_parts * a.num_kv_heads * cdiv(a.groups, kF32Rows);
   if (!a.qsl && units >= (1LL << 32) / (64 * kF32Waves)) return false;
-  return dtype == LI_F32 && !a.kv_fp8 && (a.head_dim == 64 || a.head_dim == 128) && rows_aligned(a.q, a.q_s0, a.q_s1) &&
+  return dtype == LI_F32 && !a.kv_fp8 && !a.kv_int8 && (a.head_dim == 64 || a.head_dim == 128) && rows_aligned(a.q, a.q_s0, a.q_s1) &&
          rows_aligned(a.out, a.o_s0, a.o_s1) && rows_aligned(a.kp, a.p_s0, a.p_s1) &&
          rows_aligned(a.vp, a.p_s0, a.p_s1) && a.p_s0 >= 0 && a.p_s0 < (1LL << 30);
 }

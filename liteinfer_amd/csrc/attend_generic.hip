@@ -14,16 +14,27 @@
 // One wave64 per (sequence, KV head, query block, partition); it walks the
 // block's rows (query, head) one at a time. Lane j scores key t0 + j of a
 // tile, then the tile's weights are broadcast lane to lane while each lane
-// accumulates the dims it owns (d = lane + 64 c).
+// accumulates the dims it owns (d = lane + 64 c). An int8 pool's codes take
+// their block's scale with the key's score and weight (which then stays in
+// fp32: there is no value dtype to round it to).
 #include "li_attention.h"
+
+#include <type_traits>
 
 namespace li {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <typename T>
+template <typename P>
+__device__ __forceinline__ float value_of(P x) {
+  if constexpr (std::is_same<P, int8_t>::value) return (float)(int)x;
+  else return li_to_float(x);
+}
+
+template <typename T, bool I8>
 __global__ __launch_bounds__(64) void attend_generic(AttnArgs a) {
+  using P = std::conditional_t<I8, int8_t, T>;  // pool element
   constexpr int kMaxC = kGenericMaxHeadDim / 64;
   __shared__ float qs[kGenericMaxHeadDim];
 
@@ -74,8 +85,8 @@ __global__ __launch_bounds__(64) void attend_generic(AttnArgs a) {
   }
 
   const T* qp = static_cast<const T*>(a.q);
-  const T* kpool = static_cast<const T*>(a.kp) + (int64_t)kvh * a.p_s1;
-  const T* vpool = static_cast<const T*>(a.vp) + (int64_t)kvh * a.p_s1;
+  const P* kpool = static_cast<const P*>(a.kp) + (int64_t)kvh * a.p_s1;
+  const P* vpool = static_cast<const P*>(a.vp) + (int64_t)kvh * a.p_s1;
   const int64_t* srow = a.st + (int64_t)seq * a.st_s;
   const int D = a.head_dim;
   const int bkv = min(max(a.block_kv, 1), 64);
@@ -99,18 +110,23 @@ __global__ __launch_bounds__(64) void attend_generic(AttnArgs a) {
         const int key = t0 + lane;
         const bool valid = lane < bkv && key < kend;
         int64_t slot = valid ? srow[key] : 0;
-        float s = -INFINITY;
+        float s = -INFINITY, vscale = 0.f;
         if (valid) {
-          const T* kr = kpool + slot * a.p_s0;
+          const P* kr = kpool + slot * a.p_s0;
           float dot = 0.f;
-          for (int d = 0; d < D; ++d) dot = fmaf(qs[d], li_to_float(kr[d]), dot);
+          for (int d = 0; d < D; ++d) dot = fmaf(qs[d], value_of(kr[d]), dot);
           s = dot * a.scale;
+          if constexpr (I8) {
+            const int64_t at = slot / a.block_size * a.sc_s + kvh;
+            s *= a.ks[at];
+            vscale = a.vs[at];
+          }
         }
         const float mnew = fmaxf(m, li_wave_max(s));
         const float alpha = (m == -INFINITY) ? 0.f : expf(m - mnew);
         const float p = valid ? expf(s - mnew) : 0.f;
         l = l * alpha + li_wave_sum(p);
-        const float pv = li_to_float(li_from_float<T>(p));
+        const float pv = I8 ? (valid ? p * vscale : 0.f) : li_to_float(li_from_float<T>(p));
 #pragma unroll
         for (int c = 0; c < kMaxC; ++c) acc[c] *= alpha;
         const int nvalid = min(bkv, kend - t0);
@@ -119,11 +135,11 @@ __global__ __launch_bounds__(64) void attend_generic(AttnArgs a) {
         for (int j = 0; j < nvalid; ++j) {
           const float pj = __shfl(pv, j, 64);
           const int64_t sj = ((int64_t)__shfl(slot_hi, j, 64) << 32) | (uint32_t)__shfl(slot_lo, j, 64);
-          const T* vr = vpool + sj * a.p_s0;
+          const P* vr = vpool + sj * a.p_s0;
 #pragma unroll
           for (int c = 0; c < kMaxC; ++c) {
             const int d = lane + 64 * c;
-            if (d < D) acc[c] = fmaf(pj, li_to_float(vr[d]), acc[c]);
+            if (d < D) acc[c] = fmaf(pj, value_of(vr[d]), acc[c]);
           }
         }
         m = mnew;
@@ -224,12 +240,18 @@ int launch_attend_generic(const AttnArgs& a, int dtype, hipStream_t s) {
   const int64_t blocks = (int64_t)a.batch * a.num_qblocks * a.num_kv_heads * a.num_parts;
   if (blocks == 0) return LI_OK;
   if (blocks > 0xffffffffLL) return fail(LI_EUNSUPPORTED, "attention grid of %lld blocks is too large", (long long)blocks);
+#define LI_GENERIC(T)                                                                                           \
+  do {                                                                                                          \
+    if (a.kv_int8) hipLaunchKernelGGL((attend_generic<T, true>), dim3((unsigned)blocks), dim3(64), 0, s, a);    \
+    else hipLaunchKernelGGL((attend_generic<T, false>), dim3((unsigned)blocks), dim3(64), 0, s, a);             \
+  } while (0)
   switch (dtype) {
-    case LI_F32: hipLaunchKernelGGL(attend_generic<float>, dim3((unsigned)blocks), dim3(64), 0, s, a); break;
-    case LI_F16: hipLaunchKernelGGL(attend_generic<li_f16>, dim3((unsigned)blocks), dim3(64), 0, s, a); break;
-    case LI_BF16: hipLaunchKernelGGL(attend_generic<li_bf16>, dim3((unsigned)blocks), dim3(64), 0, s, a); break;
+    case LI_F32: LI_GENERIC(float); break;
+    case LI_F16: LI_GENERIC(li_f16); break;
+    case LI_BF16: LI_GENERIC(li_bf16); break;
     default: return fail(LI_EINVAL, "unknown dtype %d", dtype);
   }
+#undef LI_GENERIC
   return check_launch("attend_generic");
 }
 

@@ -66,6 +66,14 @@ struct AttnArgs {
   // the query's dtype and ignore the scales.
   int kv_fp8;
   float k_scale, v_scale;
+  // int8 pools: kp / vp hold codes, one byte per element (pool strides in
+  // bytes), slot s of KV head h standing for code * ks[s / block_size * sc_s
+  // + h] (vs for V).
+  int kv_int8;
+  const float* ks;
+  const float* vs;
+  int64_t sc_s;
+  int block_size;
   // Head-grouped decode over a 16-bit pool: each sequence's newest K / V
   // rows, [batch, num_kv_heads, head_dim] with element strides (n_s0, n_s1,
   // 1), written to slot st[seq, ctx - 1] by the wave that folds that key

@@ -150,6 +150,32 @@ int check_common(int dtype, int num_heads, int num_kv_heads, int head_dim, const
   return LI_OK;
 }
 
+// An int8 pool's scales and blocks (AttnArgs::ks).
+struct BlockScales {
+  const float* k;
+  const float* v;
+  int64_t stride;
+  int block_size;
+};
+
+int check_block_scales(const BlockScales& sc, int num_kv_heads, const char* who) {
+  if (!sc.k || !sc.v) return fail(LI_EINVAL, "%s: null scales", who);
+  if (sc.block_size < 1 || sc.block_size > LI_INT8_MAX_BLOCK)
+    return fail(LI_EUNSUPPORTED, "%s: blocks of %d slots are outside 1..%d", who, sc.block_size, LI_INT8_MAX_BLOCK);
+  if (sc.stride < num_kv_heads)
+    return fail(LI_EINVAL, "%s: a scale stride of %lld overlaps rows of %d heads", who, (long long)sc.stride,
+                num_kv_heads);
+  return LI_OK;
+}
+
+void set_block_scales(AttnArgs& a, const BlockScales& sc) {
+  a.kv_int8 = 1;
+  a.ks = sc.k;
+  a.vs = sc.v;
+  a.sc_s = sc.stride;
+  a.block_size = sc.block_size;
+}
+
 // li_paged_decode_write's newest K / V rows: [batch, num_kv_heads, head_dim]
 // with element strides (s0, s1, 1), for slot slot_table[i, ctx[i] - 1].
 struct NewestRows {
@@ -237,10 +263,13 @@ int paged_decode_impl(const void* q, int64_t q_stride_seq, int64_t q_stride_head
                       const int32_t* context_lens, void* out, int64_t out_stride_seq, int64_t out_stride_head,
                       int batch, int num_heads, int num_kv_heads, int head_dim, float scale, int num_splits,
                       int block_kv, void* workspace, size_t workspace_bytes, int dtype, int kv_dtype, float k_scale,
-                      float v_scale, int flags, void* stream, const NewestRows* newest = nullptr) {
+                      float v_scale, int flags, void* stream, const NewestRows* newest = nullptr,
+                      const BlockScales* scales = nullptr) {
   clear_error();
   if (int rc = check_common(dtype, num_heads, num_kv_heads, head_dim, "li_paged_decode")) return rc;
   if (int rc = check_kv(dtype, kv_dtype, k_scale, v_scale, "li_paged_decode")) return rc;
+  if (scales)
+    if (int rc = check_block_scales(*scales, num_kv_heads, "li_paged_decode_int8")) return rc;
   if (num_splits < 0) return fail(LI_EINVAL, "num_splits must be >= 1, got %d", num_splits);
   if (batch < 0 || max_context < 0) return fail(LI_EINVAL, "li_paged_decode: negative extent");
   if (batch == 0) return LI_OK;
@@ -284,6 +313,7 @@ int paged_decode_impl(const void* q, int64_t q_stride_seq, int64_t q_stride_head
   a.kv_fp8 = kv_dtype == LI_FP8_E4M3;
   a.k_scale = k_scale;
   a.v_scale = v_scale;
+  if (scales) set_block_scales(a, *scales);
   if (parts > 1) {
     const size_t rows = (size_t)batch * num_heads * parts;
     a.part_o = static_cast<float*>(workspace);
@@ -400,6 +430,21 @@ extern "C" int li_paged_decode_write(const void* q, int64_t q_stride_seq, int64_
                            slot_table, slot_table_stride, max_context, context_lens, out, out_stride_seq,
                            out_stride_head, batch, num_heads, num_kv_heads, head_dim, scale, num_splits, block_kv,
                            workspace, workspace_bytes, dtype, kv_dtype, k_scale, v_scale, flags, stream, &newest);
+}
+
+extern "C" int li_paged_decode_int8(const void* q, int64_t q_stride_seq, int64_t q_stride_head, const void* key_pool,
+                                    const void* value_pool, const float* key_scales, const float* value_scales,
+                                    int block_size, int64_t scale_stride_block, int64_t pool_stride_slot,
+                                    int64_t pool_stride_head, const int64_t* slot_table, int64_t slot_table_stride,
+                                    int max_context, const int32_t* context_lens, void* out, int64_t out_stride_seq,
+                                    int64_t out_stride_head, int batch, int num_heads, int num_kv_heads, int head_dim,
+                                    float scale, int num_splits, int block_kv, void* workspace, size_t workspace_bytes,
+                                    int dtype, int flags, void* stream) {
+  const BlockScales scales{key_scales, value_scales, scale_stride_block, block_size};
+  return paged_decode_impl(q, q_stride_seq, q_stride_head, key_pool, value_pool, pool_stride_slot, pool_stride_head,
+                           slot_table, slot_table_stride, max_context, context_lens, out, out_stride_seq,
+                           out_stride_head, batch, num_heads, num_kv_heads, head_dim, scale, num_splits, block_kv,
+                           workspace, workspace_bytes, dtype, dtype, 1.f, 1.f, flags, stream, nullptr, &scales);
 }
 
 // The no-allocation decode: the workspace li_paged_decode would take lives in
@@ -534,10 +579,13 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
                        const int32_t* context_lens, const int32_t* query_start_loc, int batch, int max_query_len,
                        void* out, int64_t out_stride_tok, int64_t out_stride_head, int num_heads, int num_kv_heads,
                        int head_dim, float scale, int block_q, int block_kv, void* workspace, size_t workspace_bytes,
-                       int dtype, int kv_dtype, float k_scale, float v_scale, int flags, void* stream) {
+                       int dtype, int kv_dtype, float k_scale, float v_scale, int flags, void* stream,
+                       const BlockScales* scales = nullptr) {
   clear_error();
   if (int rc = check_common(dtype, num_heads, num_kv_heads, head_dim, "li_paged_prefill")) return rc;
   if (int rc = check_kv(dtype, kv_dtype, k_scale, v_scale, "li_paged_prefill")) return rc;
+  if (scales)
+    if (int rc = check_block_scales(*scales, num_kv_heads, "li_paged_prefill_int8")) return rc;
   if (batch < 0 || max_query_len < 0 || max_context < 0) return fail(LI_EINVAL, "li_paged_prefill: negative extent");
   if (batch == 0 || max_query_len == 0) return LI_OK;
   if (!q || !key_pool || !value_pool || !slot_table || !context_lens || !query_start_loc || !out)
@@ -572,6 +620,7 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
   a.kv_fp8 = kv_dtype == LI_FP8_E4M3;
   a.k_scale = k_scale;
   a.v_scale = v_scale;
+  if (scales) set_block_scales(a, *scales);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool mfma = !(flags & LI_FLAG_FORCE_GENERIC) && prefill_mfma_applies(a, dtype);
@@ -663,4 +712,34 @@ extern "C" int li_paged_prefill_ex(const void* q, int64_t q_stride_tok, int64_t 
                             max_query_len, out, out_stride_tok, out_stride_head, num_heads, num_kv_heads, head_dim,
                             scale, block_q, block_kv, workspace, workspace_bytes, dtype, kv_dtype, k_scale, v_scale,
                             flags, stream);
+}
+
+extern "C" int li_paged_prefill_int8_plan(int batch, int num_heads, int num_kv_heads, int head_dim, int max_context,
+                                          int max_query_len, int64_t context_tokens, int dtype,
+                                          size_t* workspace_bytes) {
+  clear_error();
+  if (int rc = check_common(dtype, num_heads, num_kv_heads, head_dim, "li_paged_prefill_int8_plan")) return rc;
+  if (batch < 0 || max_context < 0 || max_query_len < 0 || context_tokens < 0)
+    return fail(LI_EINVAL, "li_paged_prefill_int8_plan: negative extent");
+  if (workspace_bytes) *workspace_bytes = 0;
+  return LI_OK;
+}
+
+extern "C" int li_paged_prefill_int8(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* key_pool,
+                                     const void* value_pool, const float* key_scales, const float* value_scales,
+                                     int block_size, int64_t scale_stride_block, int64_t pool_stride_slot,
+                                     int64_t pool_stride_head, const int64_t* slot_table, int64_t slot_table_stride,
+                                     int max_context, const int32_t* context_lens, const int32_t* query_start_loc,
+                                     int batch, int max_query_len, int64_t context_tokens, void* out,
+                                     int64_t out_stride_tok, int64_t out_stride_head, int num_heads, int num_kv_heads,
+                                     int head_dim, float scale, int block_q, int block_kv, void* workspace,
+                                     size_t workspace_bytes, int dtype, int flags, void* stream) {
+  clear_error();
+  if (context_tokens < 0) return fail(LI_EINVAL, "li_paged_prefill_int8: negative extent");
+  const BlockScales scales{key_scales, value_scales, scale_stride_block, block_size};
+  return paged_prefill_impl(q, q_stride_tok, q_stride_head, key_pool, value_pool, pool_stride_slot, pool_stride_head,
+                            slot_table, slot_table_stride, max_context, context_lens, query_start_loc, batch,
+                            max_query_len, out, out_stride_tok, out_stride_head, num_heads, num_kv_heads, head_dim,
+                            scale, block_q, block_kv, workspace, workspace_bytes, dtype, dtype, 1.f, 1.f, flags,
+                            stream, &scales);
 }

@@ -1664,6 +1664,7 @@ bool prefill_mfma_applies(const AttnArgs& a, int dtype) {
   if (dtype != LI_BF16 && dtype != LI_F16) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.kv_fp8 && a.head_dim != 128) return false;
+  if (a.kv_int8) return false;
   if (a.groups < 1 || a.groups > 16) return false;
   const int pe = a.kv_fp8 ? 1 : 2;
   return rows_aligned(a.q, a.q_s0, a.q_s1, 2) && rows_aligned(a.out, a.o_s0, a.o_s1, 2) &&

@@ -141,6 +141,8 @@ def _kv_dtype_code(query: torch.Tensor, key_pool: torch.Tensor, k_scale: float, 
             raise ValueError(f"an fp8 pool is read with bfloat16 or float16 queries, not {query.dtype}")
         _check_scales(k_scale, v_scale)
         return _native.LI_FP8_E4M3
+    if key_pool.dtype == torch.int8:
+        return _native.dtype_code(query.dtype)
     if query.dtype != key_pool.dtype:
         raise ValueError(f"query dtype {query.dtype} does not match the pool's {key_pool.dtype}")
     return _native.dtype_code(query.dtype)
@@ -364,6 +366,8 @@ def paged_decode(
     v_scale: float = 1.0,
     new_key: torch.Tensor | None = None,
     new_value: torch.Tensor | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attend one query per sequence over the KV each sequence's slots address.
 
@@ -402,11 +406,16 @@ def paged_decode(
             launch first elsewhere. That slot
             must belong to no other sequence's context in the call (as every
             slot a `KVCache` hands out does).
+        key_scales, value_scales: an int8 pool's scales (`kv_scatter`),
+            float32 ``[num_blocks, num_kv_heads]``: the attention is over the
+            codes times the scales of their blocks. Such a pool takes its
+            newest rows through `kv_scatter` or `rope_kv_write` before the
+            call (no `new_key` / `new_value`).
 
     Returns:
         ``[batch, num_heads, head_dim]``, same dtype as ``query``.
     """
-    if query.is_cuda and kernel in _FLAGS and (num_splits is None or num_splits > 0):
+    if query.is_cuda and key_scales is None and kernel in _FLAGS and (num_splits is None or num_splits > 0):
         # Operands that need no conversion: checked and passed on in C++.
         out = _native.fast_calls().decode(
             query, key_pool, value_pool, slot_table, context_lens, scaling, num_kv_groups, block_kv, num_splits or 0,
@@ -420,6 +429,9 @@ def paged_decode(
     batch, num_heads, head_dim = query.shape
     num_kv_heads = key_pool.shape[1]
     max_context = slot_table.shape[1]
+    block = check_block_scales(key_pool, key_scales, value_scales)
+    if block and (new_key is not None or new_value is not None):
+        raise ValueError("an int8 pool takes its newest rows through kv_scatter or rope_kv_write, not new_key / new_value")
     if (new_key is None) != (new_value is None):
         raise ValueError("give both new_key and new_value, or neither")
     if new_key is not None:
@@ -437,6 +449,19 @@ def paged_decode(
                                    device.index or 0, block_kv)
     out = torch.empty_like(query)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if block:
+        status = _native.on_device(
+            device, lib.li_paged_decode_int8,
+            query.data_ptr(), query.stride(0), query.stride(1),
+            key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+            block, max(key_scales.stride(0), num_kv_heads), key_pool.stride(0), key_pool.stride(1),
+            slot_table.data_ptr(), slot_table.stride(0), max_context, context_lens.data_ptr(),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            batch, num_heads, num_kv_heads, head_dim, float(scaling), num_splits or 0, block_kv,
+            workspace.data_ptr() if workspace is not None else None, need,
+            _native.dtype_code(query.dtype), _flags(kernel), _native.stream_handle(device))
+        _native.check(status, "paged_decode")
+        return out
     status = lib.li_paged_decode_write(
         query.data_ptr(), query.stride(0), query.stride(1),
         key_pool.data_ptr(), value_pool.data_ptr(), key_pool.stride(0), key_pool.stride(1),
@@ -480,7 +505,7 @@ def paged_decode_noalloc(
     """
     device, query, slot_table, context_lens, kv_code = _decode_inputs(
         query, key_pool, value_pool, slot_table, context_lens, num_kv_groups, num_splits, 1.0, 1.0)
-    if kv_code != _native.dtype_code(query.dtype):
+    if kv_code != _native.dtype_code(query.dtype) or key_pool.dtype == torch.int8:
         raise ValueError("paged_decode_noalloc takes a pool of the query's dtype")
     if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1:
         raise ValueError("out must match the query's shape, dtype and device, with a contiguous last axis")
@@ -528,6 +553,9 @@ def paged_prefill(
     k_scale: float = 1.0,
     v_scale: float = 1.0,
     out: torch.Tensor | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    context_tokens: int | None = None,
 ) -> torch.Tensor:
     """Attend each sequence's chunk of queries over the KV its slots address, causally.
 
@@ -558,12 +586,18 @@ def paged_prefill(
         k_scale, v_scale: the scales of an fp8 pool (see `paged_decode`).
         out: where to write the result (the query's shape and dtype, last
             axis contiguous, any other strides); a new tensor when None.
+        key_scales, value_scales: an int8 pool's scales (see `paged_decode`).
+            The MFMA kernels then read the chunks' contexts from a copy in the
+            query's dtype that the call makes, as the dense kernels gather them.
+        context_tokens: the sum of `context_lens` where the host knows it
+            (an int8 pool's copy holds as many rows; None: batch times the
+            table's width). Less than the sum leaves the result unspecified.
 
     Returns:
         ``[total_queries, num_heads, head_dim]`` (`out`, or a new tensor with
         the strides of `query`).
     """
-    if query.is_cuda and kernel in ("auto", "generic"):
+    if query.is_cuda and key_scales is None and kernel in ("auto", "generic"):
         # Operands that need no conversion: checked and passed on in C++.
         flags = _FLAGS[kernel] | (_native.LI_FLAG_PREFILL_ONLY if one_query_rows is False else 0)
         got = _native.fast_calls().prefill(
@@ -598,13 +632,40 @@ def paged_prefill(
     max_context = slot_table.shape[1]
 
     lib = _native.load()
-    need = _prefill_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_context, device.index or 0)
+    block = check_block_scales(key_pool, key_scales, value_scales)
+    if block:
+        if context_tokens is not None and context_tokens < 0:
+            raise ValueError(f"context_tokens must be >= 0, got {context_tokens}")
+        tokens = batch * max_context if context_tokens is None else int(context_tokens)
+        need = _native.ctypes.c_size_t()
+        _native.check(_native.on_device(
+            device, lib.li_paged_prefill_int8_plan, batch, num_heads, num_kv_heads, head_dim, max_context,
+            int(max_query_len), tokens, _native.dtype_code(query.dtype), _native.ctypes.byref(need)), "paged_prefill")
+        need = need.value
+    else:
+        need = _prefill_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_context, device.index or 0)
     if out is None:
         out = torch.empty_like(query)
     elif (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
           or out.stride(-1) != 1):
         raise ValueError("out must match the query's shape, dtype and device, with a contiguous last axis")
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if block:
+        status = _native.on_device(
+            device, lib.li_paged_prefill_int8,
+            query.data_ptr(), query.stride(0), query.stride(1),
+            key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+            block, max(key_scales.stride(0), num_kv_heads), key_pool.stride(0), key_pool.stride(1),
+            slot_table.data_ptr(), slot_table.stride(0), max_context,
+            context_lens.data_ptr(), query_start_loc.data_ptr(), batch, int(max_query_len), tokens,
+            out.data_ptr(), out.stride(0), out.stride(1),
+            num_heads, num_kv_heads, head_dim, float(scaling), block_q, block_kv,
+            workspace.data_ptr() if workspace is not None else None, need,
+            _native.dtype_code(query.dtype),
+            _flags(_prefill_kernel(kernel)) | (_native.LI_FLAG_PREFILL_ONLY if one_query_rows is False else 0),
+            _native.stream_handle(device))
+        _native.check(status, "paged_prefill")
+        return out
     status = lib.li_paged_prefill_ex(
         query.data_ptr(), query.stride(0), query.stride(1),
         key_pool.data_ptr(), value_pool.data_ptr(), key_pool.stride(0), key_pool.stride(1),
