@@ -22,10 +22,10 @@ constexpr int kCombineWaves = LI_COMBINE_WAVES;
 // pinned split count (the reference's equal-slice rule: partition p of a
 // context of c keys is [p * cdiv(c, S), ...)).
 // ---------------------------------------------------------------------------
-template <typename T, int D, bool F8>
+template <typename T, int D, int KV>
 __global__ __launch_bounds__(64) void decode_partitioned(AttnArgs a) {
-  __shared__ __attribute__((aligned(1024))) DecodeLds<D, F8> lds;
-  const float vscale = F8 ? a.v_scale : 1.f;
+  __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds;
+  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   // Partition-major order: every sequence's first partition is dispatched
   // before any second one, so the grid's empty tail comes last.
   int bid = blockIdx.x;
@@ -51,11 +51,11 @@ __global__ __launch_bounds__(64) void decode_partitioned(AttnArgs a) {
   const int ke = min(kb + plen, ctx);
   const int nparts = (ctx + plen - 1) / plen;
 
-  DecodeQuery<T, D, F8> q;
+  DecodeQuery<T, D, KV> q;
   load_query(a, row, kvh, q);
   DecodeState st;
   reset_state(st);
-  fold_keys<T, D, F8>(a, lds, q, seq, kvh, kb, ke, st);
+  fold_keys<T, D, KV>(a, lds, q, seq, kvh, kb, ke, st);
   const int head0 = kvh * a.groups;
   if (nparts == 1) {
     store_state<T, D>(st, static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)head0 * a.o_s1, a.o_s1,
@@ -67,10 +67,10 @@ __global__ __launch_bounds__(64) void decode_partitioned(AttnArgs a) {
   }
 }
 
-template <typename T, int D, bool F8>
+template <typename T, int D, int KV>
 __global__ __launch_bounds__(64) void decode_balanced(AttnArgs a) {
-  __shared__ __attribute__((aligned(1024))) DecodeLds<D, F8> lds;
-  decode_balanced_wave<T, D, F8>(a, (int)blockIdx.x, a.num_parts, lds);
+  __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds;
+  decode_balanced_wave<T, D, KV>(a, (int)blockIdx.x, a.num_parts, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -91,17 +91,18 @@ __global__ __launch_bounds__(64) void decode_balanced(AttnArgs a) {
 // segment's 32-key tiles plus AttnArgs::seg_cost for starting it), not in
 // keys.
 // ---------------------------------------------------------------------------
-template <typename T, int D, bool F8, int HG, int P>
+template <typename T, int D, int KV, int HG, int P>
 __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
-  using L = KvTile<D, F8>;
+  using L = KvTile<D, KV>;
+  constexpr int kChunk = kChunkOf<KV>;
   static_assert(HG % 2 == 0, "an even head count keeps every ring stage index a constant");
-  __shared__ __attribute__((aligned(1024))) DecodeLds<D, F8> lds_of[P];
-  const float vscale = F8 ? a.v_scale : 1.f;
+  __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds_of[P];
+  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   const int lane = threadIdx.x & 63;
   // Wave pw of the work-group folds head group P * grp + pw: the P waves
   // of a work-group walk the same keys of adjacent groups.
   const int pw = P > 1 ? (int)(threadIdx.x >> 6) : 0;
-  DecodeLds<D, F8>& lds = lds_of[pw];
+  DecodeLds<D, KV>& lds = lds_of[pw];
   const int w = blockIdx.x;
   const int ngroups = a.num_kv_heads / (HG * P);
   // Work is counted in units: a segment (sequence, group of HG KV heads)
@@ -162,10 +163,10 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
   }
 
   const int G = a.groups;
-  const TileOffsets<D, F8> off;
-  const int esize = F8 ? 1 : (int)sizeof(T);
+  const TileOffsets<D, KV> off;
+  const int esize = kPoolBytes<T, KV>;
   const uint32_t row_bytes = (uint32_t)(a.p_s0 * esize);
-  const float sc = a.scale * (F8 ? a.k_scale : 1.f) * kLog2eMfma;
+  const float sc = a.scale * (KV == kPoolF8 ? a.k_scale : 1.f) * kLog2eMfma;
   const int64_t head_bytes = a.p_s1 * esize;
   // Partial rows of slot s: ((w * 2 + s) * P + pw) * HG * G onwards.
   float* part_o = a.part_o + ((int64_t)w * 2 * P + pw) * HG * G * a.head_dim;
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
             int4{w, (int)((seg + nu - 1) / share), first_segment ? 0 : 1, 0};
       }
       const int row = decode_row(a, seq);
-      DecodeQuery<T, D, F8> q[HG];
+      DecodeQuery<T, D, KV> q[HG];
       DecodeState st[HG];
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
       bool write_new = false;
       u32x4_t new_row = {0u, 0u, 0u, 0u};
       int64_t new_slot = 0;
-      if constexpr (!F8) {
+      if constexpr (KV == kPool16) {
         write_new = a.new_k != nullptr && ke == ctx;
         if (write_new) {
           new_slot = srow[ctx - 1];
@@ -224,30 +225,34 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
           }
         }
       }
-      for (int c0 = kb; c0 < ke; c0 += kSlotChunk) {
-        const int c1 = min(c0 + kSlotChunk, ke);
+      for (int c0 = kb; c0 < ke; c0 += kChunk) {
+        const int c1 = min(c0 + kChunk, ke);
         const int ntiles = (c1 - c0 + 31) / 32;
         {
-          int vals[kSlotChunk / 64 + 1];
+          int vals[kChunk / 64 + 1];
 #pragma unroll
-          for (int k = 0; k < kSlotChunk / 64 + 1; ++k) vals[k] = (int)srow[min(c0 + lane + 64 * k, c1 - 1)];
+          for (int k = 0; k < kChunk / 64 + 1; ++k) vals[k] = (int)srow[min(c0 + lane + 64 * k, c1 - 1)];
 #pragma unroll
-          for (int k = 0; k < kSlotChunk / 64 + 1; ++k) lds.sl[lane + 64 * k] = vals[k];
+          for (int k = 0; k < kChunk / 64 + 1; ++k) lds.sl[lane + 64 * k] = vals[k];
+        }
+        if constexpr (KV == kPoolI8) {
+          static_assert(HG <= kScaleHeads, "the LDS holds the scales of a group's heads");
+          stage_scales(a, lds, h0, HG);
         }
         // The ring runs over (tile, head) pairs; pair ti * HG + h folds from
         // stage h % 2 while the next pair's loads land in the other stage.
         // Past the chunk the look-ahead re-reads a real tile.
         constexpr int kInFlight = 2 * L::kInsts;
-        issue_tile<D, F8>(lds.stage[0], kbase, vbase, lds.sl, row_bytes, 0, lane);
+        issue_tile<D, KV>(lds.stage[0], kbase, vbase, lds.sl, row_bytes, 0, lane);
         for (int ti = 0; ti < ntiles; ++ti) {
 #pragma unroll
           for (int h = 0; h < HG; ++h) {
             const int nh = h + 1 < HG ? h + 1 : 0;
             const int nt = h + 1 < HG ? ti : ti + 1;
-            issue_tile<D, F8>(lds.stage[(h + 1) & 1], kbase + nh * head_bytes, vbase + nh * head_bytes, lds.sl,
-                              row_bytes, min(32 * nt, kSlotChunk), lane);
+            issue_tile<D, KV>(lds.stage[(h + 1) & 1], kbase + nh * head_bytes, vbase + nh * head_bytes, lds.sl,
+                              row_bytes, min(32 * nt, kChunk), lane);
             li_wait_vm<kInFlight>();
-            if constexpr (!F8) {
+            if constexpr (KV == kPool16) {
               const int tk = c0 + 32 * ti;  // the tile's first key
               if (write_new && tk + 32 >= ctx) {
                 // The tile holding key ctx - 1: its row, and the rows past it
@@ -264,7 +269,11 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
               }
             }
-            fold_tile<T, D, F8>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h]);
+            if constexpr (KV == kPoolI8)
+              fold_tile<T, D, KV>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h],
+                                  lds.ks[h] + 32 * ti, lds.vs[h] + 32 * ti);
+            else
+              fold_tile<T, D, KV>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h]);
           }
         }
         li_wait_vm<0>();
@@ -534,9 +543,9 @@ __global__ __launch_bounds__(64 * NW) void combine_wide(AttnArgs a) {
 // combine launch: a call is its loads' round trips and one launch. Over a
 // 16-bit pool it also writes the step's newest K / V rows (a.new_k).
 // ---------------------------------------------------------------------------
-template <typename T, int D, bool F8, int NW>
+template <typename T, int D, int KV, int NW>
 __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
-  using Lds = DecodeLds<D, F8, kShortChunk>;
+  using Lds = DecodeLds<D, KV, kShortChunk>;
   static_assert(sizeof(Lds::stage) >= 16 * D * sizeof(float), "a wave's state fits its stages");
   __shared__ __attribute__((aligned(1024))) Lds lds_of[NW];
   __shared__ float s_m[NW][16], s_l[NW][16];
@@ -550,7 +559,7 @@ __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
   // Wave wv's run: [wv * per, (wv + 1) * per) of the context, whole tiles.
   const int per = ((keys + NW - 1) / NW + 31) / 32 * 32;
   const int kb = min(wv * per, keys), ke = min(kb + per, keys);
-  if constexpr (!F8) {
+  if constexpr (KV == kPool16) {
     if (a.new_k != nullptr && kb < ke && ke == keys) {
       // This wave folds the context's last key: the step's new K and V rows
       // of this KV head go to that key's slot first (lane (kv, c) stores
@@ -577,9 +586,9 @@ __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
   DecodeState st;
   reset_state(st);
   if (ke > kb) {
-    DecodeQuery<T, D, F8> q;
+    DecodeQuery<T, D, KV> q;
     load_query(a, row, kvh, q);
-    fold_keys<T, D, F8>(a, lds_of[wv], q, seq, kvh, kb, ke, st);
+    fold_keys<T, D, KV>(a, lds_of[wv], q, seq, kvh, kb, ke, st);
   }
   // Each wave's state into its own stages (its loads have drained): head n's
   // accumulator row, its running maximum and its denominator.
@@ -596,7 +605,7 @@ __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
     }
   }
   __syncthreads();
-  const float vscale = F8 ? a.v_scale : 1.f;
+  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   T* orow = static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)kvh * G * a.o_s1;
   for (int e = threadIdx.x; e < G * D; e += 64 * NW) {
     const int h = e / D, d = e % D;
@@ -631,9 +640,8 @@ bool decode_mfma_applies(const AttnArgs& a, int dtype) {
   if (dtype != LI_BF16 && dtype != LI_F16) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.kv_fp8 && a.head_dim != 128) return false;
-  if (a.kv_int8) return false;
   if (a.groups < 1 || a.groups > 16) return false;
-  const int pe = a.kv_fp8 ? 1 : 2;
+  const int pe = a.kv_fp8 || a.kv_int8 ? 1 : 2;
   return rows_aligned(a.q, a.q_s0, a.q_s1, 2) && rows_aligned(a.out, a.o_s0, a.o_s1, 2) &&
          rows_aligned(a.kp, a.p_s0, a.p_s1, pe) && rows_aligned(a.vp, a.p_s0, a.p_s1, pe);
 }
@@ -644,26 +652,34 @@ int launch_decode_mfma(const AttnArgs& a, int dtype, hipStream_t s) {
   if (blocks == 0) return LI_OK;
   if (blocks > 0x7fffffffLL) return fail(LI_EUNSUPPORTED, "decode grid of %lld blocks is too large", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(64);
-#define LI_DECODE_LAUNCH(T, D, F8)                                                                   \
+#define LI_DECODE_LAUNCH(T, D, KV)                                                                   \
   do {                                                                                               \
     if (balanced && a.part_heads == kDecodeHeadGroup)                                                \
-      hipLaunchKernelGGL((decode_grouped<T, D, F8, kDecodeHeadGroup, 1>), grid, block, 0, s, a);     \
+      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 1>), grid, block, 0, s, a);     \
     else if (balanced && a.part_heads == 2 * kDecodeHeadGroup)                                       \
-      hipLaunchKernelGGL((decode_grouped<T, D, F8, kDecodeHeadGroup, 2>), grid, dim3(128), 0, s, a); \
+      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 2>), grid, dim3(128), 0, s, a); \
     else if (balanced && a.part_heads == 4 * kDecodeHeadGroup)                                       \
-      hipLaunchKernelGGL((decode_grouped<T, D, F8, kDecodeHeadGroup, 4>), grid, dim3(256), 0, s, a); \
-    else if (balanced) hipLaunchKernelGGL((decode_balanced<T, D, F8>), grid, block, 0, s, a);        \
-    else hipLaunchKernelGGL((decode_partitioned<T, D, F8>), grid, block, 0, s, a);                   \
+      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 4>), grid, dim3(256), 0, s, a); \
+    else if (balanced) hipLaunchKernelGGL((decode_balanced<T, D, KV>), grid, block, 0, s, a);        \
+    else hipLaunchKernelGGL((decode_partitioned<T, D, KV>), grid, block, 0, s, a);                   \
   } while (0)
   if (a.kv_fp8) {
-    if (dtype == LI_BF16) LI_DECODE_LAUNCH(li_bf16, 128, true);
-    else LI_DECODE_LAUNCH(li_f16, 128, true);
+    if (dtype == LI_BF16) LI_DECODE_LAUNCH(li_bf16, 128, kPoolF8);
+    else LI_DECODE_LAUNCH(li_f16, 128, kPoolF8);
+  } else if (a.kv_int8) {
+    if (dtype == LI_BF16) {
+      if (a.head_dim == 128) LI_DECODE_LAUNCH(li_bf16, 128, kPoolI8);
+      else LI_DECODE_LAUNCH(li_bf16, 64, kPoolI8);
+    } else {
+      if (a.head_dim == 128) LI_DECODE_LAUNCH(li_f16, 128, kPoolI8);
+      else LI_DECODE_LAUNCH(li_f16, 64, kPoolI8);
+    }
   } else if (dtype == LI_BF16) {
-    if (a.head_dim == 128) LI_DECODE_LAUNCH(li_bf16, 128, false);
-    else LI_DECODE_LAUNCH(li_bf16, 64, false);
+    if (a.head_dim == 128) LI_DECODE_LAUNCH(li_bf16, 128, kPool16);
+    else LI_DECODE_LAUNCH(li_bf16, 64, kPool16);
   } else {
-    if (a.head_dim == 128) LI_DECODE_LAUNCH(li_f16, 128, false);
-    else LI_DECODE_LAUNCH(li_f16, 64, false);
+    if (a.head_dim == 128) LI_DECODE_LAUNCH(li_f16, 128, kPool16);
+    else LI_DECODE_LAUNCH(li_f16, 64, kPool16);
   }
 #undef LI_DECODE_LAUNCH
   if (int rc = check_launch("decode_mfma")) return rc;
@@ -690,14 +706,22 @@ int launch_decode_short(const AttnArgs& a, int dtype, hipStream_t s) {
   const dim3 grid((unsigned)blocks);
   // Waves per work-group: as many as the LDS holds (two tile stages each).
   if (a.kv_fp8) {
-    if (dtype == LI_BF16) hipLaunchKernelGGL((decode_short<li_bf16, 128, true, 8>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((decode_short<li_f16, 128, true, 8>), grid, dim3(512), 0, s, a);
+    if (dtype == LI_BF16) hipLaunchKernelGGL((decode_short<li_bf16, 128, kPoolF8, 8>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((decode_short<li_f16, 128, kPoolF8, 8>), grid, dim3(512), 0, s, a);
+  } else if (a.kv_int8) {
+    if (dtype == LI_BF16) {
+      if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_bf16, 128, kPoolI8, 4>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((decode_short<li_bf16, 64, kPoolI8, 8>), grid, dim3(512), 0, s, a);
+    } else {
+      if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_f16, 128, kPoolI8, 4>), grid, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((decode_short<li_f16, 64, kPoolI8, 8>), grid, dim3(512), 0, s, a);
+    }
   } else if (dtype == LI_BF16) {
-    if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_bf16, 128, false, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((decode_short<li_bf16, 64, false, 8>), grid, dim3(512), 0, s, a);
+    if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_bf16, 128, kPool16, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((decode_short<li_bf16, 64, kPool16, 8>), grid, dim3(512), 0, s, a);
   } else {
-    if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_f16, 128, false, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((decode_short<li_f16, 64, false, 8>), grid, dim3(512), 0, s, a);
+    if (a.head_dim == 128) hipLaunchKernelGGL((decode_short<li_f16, 128, kPool16, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((decode_short<li_f16, 64, kPool16, 8>), grid, dim3(512), 0, s, a);
   }
   return check_launch("decode_short");
 }

@@ -55,20 +55,25 @@ __device__ __forceinline__ int li_lane() { return (int)(threadIdx.x & 63); }
 // lines in L2).
 constexpr bool kDecodeStream = true;
 
-// The LDS tile layout of a pool: bf16 / fp16 rows, or fp8 (e4m3) rows at
-// head_dim 128.
-template <int D, bool F8>
-using KvTile = std::conditional_t<F8, F8Tile, TileLayout<D>>;
+// The LDS tile layout of a pool: bf16 / fp16 rows, fp8 (e4m3) rows at
+// head_dim 128, or int8 codes.
+template <int D, int KV>
+using KvTile = std::conditional_t<KV == kPool16, TileLayout<D>,
+                                  std::conditional_t<KV == kPoolI8 && D == 64, I8Tile64, F8Tile>>;
+
+// Bytes per pool element.
+template <typename T, int KV>
+constexpr int kPoolBytes = KV == kPool16 ? (int)sizeof(T) : 1;
 
 // Issues the 2 * kInsts direct-to-LDS loads of the 32-key tile whose first
 // key is entry `t` of the staged slots, into the stage at `stage`. Lane
 // (rr, n) = (lane / CH, lane % CH) loads keys rr * kInsts + i. kpool / vpool
 // point at the KV head's row of slot 0, row_bytes is the pool's slot stride.
-template <int D, bool F8>
+template <int D, int KV>
 __device__ __forceinline__ void issue_tile(char* stage, const char* __restrict__ kpool,
                                            const char* __restrict__ vpool, const int* __restrict__ sl,
                                            uint32_t row_bytes, int t, int lane) {
-  using L = KvTile<D, F8>;
+  using L = KvTile<D, KV>;
   const int rr = lane / L::kCh, nn = lane % L::kCh;
   int keys[L::kInsts];
   if constexpr (L::kInsts == 8) {
@@ -76,9 +81,12 @@ __device__ __forceinline__ void issue_tile(char* stage, const char* __restrict__
     const int4 b = *reinterpret_cast<const int4*>(sl + t + 8 * rr + 4);
     keys[0] = a.x; keys[1] = a.y; keys[2] = a.z; keys[3] = a.w;
     keys[4] = b.x; keys[5] = b.y; keys[6] = b.z; keys[7] = b.w;
-  } else {
+  } else if constexpr (L::kInsts == 4) {
     const int4 a = *reinterpret_cast<const int4*>(sl + t + 4 * rr);
     keys[0] = a.x; keys[1] = a.y; keys[2] = a.z; keys[3] = a.w;
+  } else {
+    const int2 a = *reinterpret_cast<const int2*>(sl + t + 2 * rr);
+    keys[0] = a.x; keys[1] = a.y;
   }
 #pragma unroll
   for (int i = 0; i < L::kInsts; ++i) {
@@ -90,12 +98,27 @@ __device__ __forceinline__ void issue_tile(char* stage, const char* __restrict__
   }
 }
 
+// Keys a wave of the balanced and partitioned kernels stages at a time. An
+// int8 pool's chunks are shorter, as their scales are staged too.
+template <int KV>
+constexpr int kChunkOf = KV == kPoolI8 ? 256 : kSlotChunk;
+
 // LDS of one decode wave: the staged slots of a chunk of kChunk keys (a
 // multiple of 64) and two tile stages.
-template <int D, bool F8, int kChunk = kSlotChunk>
+template <int D, int KV, int kChunk = kChunkOf<KV>>
 struct DecodeLds {
   int sl[kChunk + 64];
-  char stage[2][KvTile<D, F8>::kTileBytes];
+  char stage[2][KvTile<D, KV>::kTileBytes];
+};
+// int8 pools: the staged keys' scales too, for each of the kScaleHeads KV
+// heads that the wave folds side by side.
+constexpr int kScaleHeads = kDecodeHeadGroup;
+template <int D, int kChunk>
+struct DecodeLds<D, kPoolI8, kChunk> {
+  int sl[kChunk + 64];
+  float ks[kScaleHeads][kChunk + 64];
+  float vs[kScaleHeads][kChunk + 64];
+  char stage[2][KvTile<D, kPoolI8>::kTileBytes];
 };
 
 // Online-softmax state of one wave: lane (n, g) holds head n's running max
@@ -174,35 +197,90 @@ __device__ __forceinline__ float split_e4m3(float (&x)[32], v8i_t (&t)[kTerms]) 
   return __uint_as_float((uint32_t)(127 - ex) << 23);
 }
 
-template <typename T, int D, bool F8>
+template <typename T, int D, int KV>
 struct DecodeQuery {
   typename Mfma<T>::Frag f[D / 32];
   float scale;  // 1
 };
 
 template <typename T, int D>
-struct DecodeQuery<T, D, true> {
+struct DecodeQuery<T, D, kPoolF8> {
   static_assert(D == 128, "fp8 pools: head_dim 128");
   static constexpr int kTerms = std::is_same<T, li_f16>::value ? 3 : 2;
   v8i_t t[kTerms];
   float scale;  // 2^-e
 };
 
+// int8 pools: the scores run on v_mfma_i32_16x16x64_i8 with K straight from
+// the pool, so the query is given in integers as well: head n's row times the
+// power of two that puts its largest |value| in [2^21, 2^22), rounded (22
+// bits of the row's largest value: half a step of 2^-22 of it at most), in
+// three balanced base-256 digits. The digits' integer products are exact;
+// `scale` returns the scores to the query's units (a NaN for a row that holds
+// a value that is not finite). Lane (n, g) holds bytes 64 j + 16 g .. of head
+// n for step j, the order in which it reads the codes of its key.
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+
+template <typename T, int D>
+struct DecodeQuery<T, D, kPoolI8> {
+  v4i_t t[3][D / 64];
+  float scale;
+};
+
+template <int D>
+__device__ __forceinline__ float split_i8(const float (&x)[D / 64][16], v4i_t (&t)[3][D / 64]) {
+  uint32_t top = 0;  // as bits: what is not finite orders above the rest
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+  const bool lost = top >= 0x7f800000u;
+  // top 2^ex in [2^21, 2^22); held to 2^120 (rows below 2^-99 keep fewer
+  // bits), so that the scores' factor is no denormal.
+  const int ex = top == 0 ? 0 : min(max(148 - (int)(top >> 23), -126), 120);
+  const float mult = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t d0 = 0, d1 = 0, d2 = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int v = lost ? 0 : (int)rintf(x[j][4 * w + b] * mult);
+        const int lo = (int)(int8_t)v, m = (v - lo) >> 8, mid = (int)(int8_t)m, hi = (m - mid) >> 8;
+        d0 |= (uint32_t)(hi & 255) << (8 * b);
+        d1 |= (uint32_t)(mid & 255) << (8 * b);
+        d2 |= (uint32_t)(lo & 255) << (8 * b);
+      }
+      t[0][j][w] = (int)d0;
+      t[1][j][w] = (int)d1;
+      t[2][j][w] = (int)d2;
+    }
+  return __uint_as_float(lost ? 0x7fc00000u : (uint32_t)(127 - ex) << 23);
+}
+
 // Per-lane LDS byte offsets within a tile: the K operand of key n, step j
 // (key 16 + n sits L::kRow16 bytes below), and the V^T reads' addresses
 // (li_read_vt's two for 16-bit rows, the one 8-bit transposing read for
 // fp8 rows; see F8Tile).
-template <int D, bool F8>
+template <int D, int KV>
 struct TileOffsets {
   uint32_t koff[D / 32], voff[D / 16];
-  uint32_t kq[2];  // fp8: the two 16-byte chunks (dims 32 g ..) of key n's K row
+  uint32_t kq[2];  // fp8: the two 16-byte chunks (dims 32 g ..) of key n's K row; int8: chunk 4 j + g
   __device__ __forceinline__ TileOffsets() {
-    using L = KvTile<D, F8>;
+    using L = KvTile<D, KV>;
     const int lane = li_lane();
     const int n = lane & 15, g = lane >> 4;
-    if constexpr (F8) {
-      kq[0] = L::offset(n, 2 * g);
-      kq[1] = L::offset(n, 2 * g + 1);
+    if constexpr (KV != kPool16) {
+      if constexpr (KV == kPoolF8) {
+        kq[0] = L::offset(n, 2 * g);
+        kq[1] = L::offset(n, 2 * g + 1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) kq[j] = L::offset(n, 4 * j + g);
+      }
       const int s16 = lane & 15;
 #pragma unroll
       for (int blk = 0; blk < D / 16; ++blk) voff[blk] = L::voffset(kappa(g, s16 >> 1), blk) + 8 * (s16 & 1);
@@ -219,18 +297,44 @@ struct TileOffsets {
 // Folds the 32-key tile in `stage` (LDS byte address) whose first key is t0
 // into `st`; keys at or past `te` are masked. q holds the group's query, sc
 // the softmax scale times log2(e) (and an fp8 pool's k_scale, and the
-// query's scale q.scale).
-template <typename T, int D, bool F8>
-__device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const DecodeQuery<T, D, F8>& q, float sc,
-                                          const TileOffsets<D, F8>& o, DecodeState& st) {
-  using M = Mfma<T>;
+// query's scale q.scale). ks / vs: an int8 pool's scales of the tile's keys,
+// in LDS; the weights of such a pool are rounded to bf16 whatever the query's
+// type, once times their keys' scales: fp16 could not hold those products.
+template <typename T, int D, int KV>
+__device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const DecodeQuery<T, D, KV>& q, float sc,
+                                          const TileOffsets<D, KV>& o, DecodeState& st, const float* ks = nullptr,
+                                          const float* vs = nullptr) {
+  using W = std::conditional_t<KV == kPoolI8, li_bf16, T>;  // the weights' type
+  using M = Mfma<W>;
   using Frag = typename M::Frag;
-  using L = KvTile<D, F8>;
+  using L = KvTile<D, KV>;
   constexpr int kSteps = D / 32;
   const int lane = li_lane();
   const int g = lane >> 4;
   floatx4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (F8) {
+  if constexpr (KV == kPoolI8) {
+    // Digit d's products with keys n and 16 + n, exact; the first two digits
+    // joined in integers (|sum| < 2^29).
+    v4i_t p0[3], p1[3];
+#pragma unroll
+    for (int d = 0; d < 3; ++d) p0[d] = p1[d] = v4i_t{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const v4i_t k0 = lds_read_frag<v4i_t>(stage + o.kq[j]), k1 = lds_read_frag<v4i_t>(stage + o.kq[j] + L::kRow16);
+#pragma unroll
+      for (int d = 0; d < 3; ++d) {
+        p0[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k0, q.t[d][j], p0[d], 0, 0, 0);
+        p1[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, q.t[d][j], p1[d], 0, 0, 0);
+      }
+    }
+    const floatx4_t ks0 = *reinterpret_cast<const floatx4_t*>(ks + 4 * g);
+    const floatx4_t ks1 = *reinterpret_cast<const floatx4_t*>(ks + 16 + 4 * g);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s0[r] = fmaf((float)(p0[0][r] * 256 + p0[1][r]), 256.f, (float)p0[2][r]) * ks0[r];
+      s1[r] = fmaf((float)(p1[0][r] * 256 + p1[1][r]), 256.f, (float)p1[2][r]) * ks1[r];
+    }
+  } else if constexpr (KV == kPoolF8) {
     // Keys n and 16 + n, dims 32 g .. 32 g + 31, as stored (e4m3).
     auto krow = [&](uint32_t at) {
       const u32x4_t lo = *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)(at + o.kq[0]);
@@ -239,7 +343,7 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
     };
     const v8i_t k0 = krow(stage), k1 = krow(stage + L::kRow16);
 #pragma unroll
-    for (int t = 0; t < DecodeQuery<T, D, F8>::kTerms; ++t) {
+    for (int t = 0; t < DecodeQuery<T, D, KV>::kTerms; ++t) {
       // Formats e4m3 (0) for both operands; block scales 2^0 for K, 2^-4t
       // for query term t.
       s0 = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k0, q.t[t], s0, 0, 0, 0, 127, 0, kTermScale(t));
@@ -281,34 +385,60 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
       for (int r = 0; r < 4; ++r) st.acc[i][r] *= alpha;
   }
   st.m = mnew;
+  if constexpr (KV == kPoolI8) {
+    const floatx4_t vs0 = *reinterpret_cast<const floatx4_t*>(vs + 4 * g);
+    const floatx4_t vs1 = *reinterpret_cast<const floatx4_t*>(vs + 16 + 4 * g);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] *= vs0[r];
+      p[4 + r] *= vs1[r];
+    }
+  }
   u32x4_t pw;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) pw[u] = li_pack2<T>(p[2 * u], p[2 * u + 1]);
+  for (int u = 0; u < 4; ++u) pw[u] = li_pack2<W>(p[2 * u], p[2 * u + 1]);
   const Frag pf = __builtin_bit_cast(Frag, pw);
   // O^T += V^T P^T, 16 dims at a time, V^T straight out of LDS.
   const uint32_t vstage = stage + 32 * L::kRowBytes;
 #pragma unroll
   for (int blk = 0; blk < D / 16; ++blk) {
-    if constexpr (F8) st.acc[blk] = M::mma(lds_read_f8_vt<Frag>(vstage + o.voff[blk]), pf, st.acc[blk]);
+    if constexpr (KV == kPoolI8) st.acc[blk] = M::mma(lds_read_i8_vt(vstage + o.voff[blk]), pf, st.acc[blk]);
+    else if constexpr (KV == kPoolF8) st.acc[blk] = M::mma(lds_read_f8_vt<Frag>(vstage + o.voff[blk]), pf, st.acc[blk]);
     else st.acc[blk] = M::mma(lds_read_vt<Frag>(vstage + o.voff[blk], vstage + o.voff[blk] + L::kRow16), pf, st.acc[blk]);
   }
 }
 
-// Folds keys [kb, ke) of sequence `seq`'s context for KV head `kvh` into `st`.
-template <typename T, int D, bool F8, int kChunk>
-__device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, F8, kChunk>& lds,
-                                          const DecodeQuery<T, D, F8>& q, int seq, int kvh, int kb, int ke,
-                                          DecodeState& st) {
-  using L = KvTile<D, F8>;
+// An int8 pool's scales of the first `count` staged keys (a multiple of 64)
+// for KV head `kvh` of heads kvh .. kvh + heads - 1, into LDS beside the slots.
+template <int D, int kChunk>
+__device__ __forceinline__ void stage_scales(const AttnArgs& a, DecodeLds<D, kPoolI8, kChunk>& lds, int kvh, int heads) {
   const int lane = li_lane();
-  const TileOffsets<D, F8> off;
-  const int esize = F8 ? 1 : (int)sizeof(T);  // bytes per pool element
+  const uint32_t bs = (uint32_t)a.block_size;
+#pragma unroll 4
+  for (int k = 0; k < kChunk / 64 + 1; ++k) {
+    const int64_t at = (int64_t)((uint32_t)lds.sl[lane + 64 * k] / bs) * a.sc_s + kvh;
+    for (int h = 0; h < heads; ++h) {
+      lds.ks[h][lane + 64 * k] = a.ks[at + h];
+      lds.vs[h][lane + 64 * k] = a.vs[at + h];
+    }
+  }
+}
+
+// Folds keys [kb, ke) of sequence `seq`'s context for KV head `kvh` into `st`.
+template <typename T, int D, int KV, int kChunk>
+__device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, KV, kChunk>& lds,
+                                          const DecodeQuery<T, D, KV>& q, int seq, int kvh, int kb, int ke,
+                                          DecodeState& st) {
+  using L = KvTile<D, KV>;
+  const int lane = li_lane();
+  const TileOffsets<D, KV> off;
+  const int esize = kPoolBytes<T, KV>;
   const char* kpool = static_cast<const char*>(a.kp) + (int64_t)kvh * a.p_s1 * esize;
   const char* vpool = static_cast<const char*>(a.vp) + (int64_t)kvh * a.p_s1 * esize;
   const uint32_t row_bytes = (uint32_t)(a.p_s0 * esize);
   const int64_t* srow = a.st + (int64_t)seq * a.st_s;
   // An fp8 pool stores K / k_scale: its scale multiplies the scores.
-  const float sc = a.scale * (F8 ? a.k_scale * q.scale : 1.f) * kLog2eMfma;
+  const float sc = a.scale * (KV == kPoolF8 ? a.k_scale * q.scale : KV == kPoolI8 ? q.scale : 1.f) * kLog2eMfma;
 
   for (int c0 = kb; c0 < ke; c0 += kChunk) {
     const int c1 = min(c0 + kChunk, ke);
@@ -324,9 +454,11 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, F8, kC
 #pragma unroll
       for (int k = 0; k < kChunk / 64 + 1; ++k) lds.sl[lane + 64 * k] = vals[k];
     }
+    if constexpr (KV == kPoolI8) stage_scales(a, lds, kvh, 1);
 
     auto fold = [&](uint32_t stage, int t0) __attribute__((always_inline)) {
-      fold_tile<T, D, F8>(stage, t0, c1, q, sc, off, st);
+      if constexpr (KV == kPoolI8) fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st, lds.ks[0] + (t0 - c0), lds.vs[0] + (t0 - c0));
+      else fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st);
     };
 
     // Two stages: while one tile is folded the next tile's loads land in the
@@ -334,13 +466,13 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, F8, kC
     // so the loads in flight are the same every step and no load sits under
     // a branch.
     constexpr int kInFlight = 2 * L::kInsts;
-    issue_tile<D, F8>(lds.stage[0], kpool, vpool, lds.sl, row_bytes, 0, lane);
+    issue_tile<D, KV>(lds.stage[0], kpool, vpool, lds.sl, row_bytes, 0, lane);
     for (int ti = 0;;) {
-      issue_tile<D, F8>(lds.stage[1], kpool, vpool, lds.sl, row_bytes, min(32 * (ti + 1), kChunk), lane);
+      issue_tile<D, KV>(lds.stage[1], kpool, vpool, lds.sl, row_bytes, min(32 * (ti + 1), kChunk), lane);
       li_wait_vm<kInFlight>();
       fold(lds_addr(lds.stage[0]), c0 + 32 * ti);
       if (++ti >= ntiles) break;
-      issue_tile<D, F8>(lds.stage[0], kpool, vpool, lds.sl, row_bytes, min(32 * (ti + 1), kChunk), lane);
+      issue_tile<D, KV>(lds.stage[0], kpool, vpool, lds.sl, row_bytes, min(32 * (ti + 1), kChunk), lane);
       li_wait_vm<kInFlight>();
       fold(lds_addr(lds.stage[1]), c0 + 32 * ti);
       if (++ti >= ntiles) break;
@@ -351,13 +483,24 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, F8, kC
 }
 
 // Loads the query operand of KV head `kvh`'s group for the query at `row`.
-template <typename T, int D, bool F8>
-__device__ __forceinline__ void load_query(const AttnArgs& a, int row, int kvh, DecodeQuery<T, D, F8>& q) {
+template <typename T, int D, int KV>
+__device__ __forceinline__ void load_query(const AttnArgs& a, int row, int kvh, DecodeQuery<T, D, KV>& q) {
   using Frag = typename Mfma<T>::Frag;
   const int lane = li_lane();
   const int n = lane & 15, g = lane >> 4;
   const T* qrow = static_cast<const T*>(a.q) + (int64_t)row * a.q_s0 + (int64_t)(kvh * a.groups + n) * a.q_s1;
-  if constexpr (!F8) {
+  if constexpr (KV == kPoolI8) {
+    float x[D / 64][16];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag f = (n < a.groups) ? *reinterpret_cast<const Frag*>(qrow + 64 * j + 16 * g + 8 * i) : Frag{};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j][8 * i + e] = (float)f[e];
+      }
+    q.scale = split_i8<D>(x, q.t);
+  } else if constexpr (KV == kPool16) {
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) q.f[j] = (n < a.groups) ? *reinterpret_cast<const Frag*>(qrow + 32 * j + 8 * g) : Frag{};
     q.scale = 1.f;
@@ -369,7 +512,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, int row, int kvh, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[8 * i + e] = (float)f[e];
     }
-    q.scale = split_e4m3<DecodeQuery<T, D, F8>::kTerms>(x, q.t);
+    q.scale = split_e4m3<DecodeQuery<T, D, KV>::kTerms>(x, q.t);
   }
 }
 
@@ -468,9 +611,9 @@ __device__ __forceinline__ void balanced_share(const AttnArgs& a, int64_t waves,
 }
 
 // One wave's share of the balanced split: wave w of `waves` (its LDS `lds`).
-template <typename T, int D, bool F8>
-__device__ __forceinline__ void decode_balanced_wave(const AttnArgs& a, int w, int64_t waves, DecodeLds<D, F8>& lds) {
-  const float vscale = F8 ? a.v_scale : 1.f;
+template <typename T, int D, int KV>
+__device__ __forceinline__ void decode_balanced_wave(const AttnArgs& a, int w, int64_t waves, DecodeLds<D, KV>& lds) {
+  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   const int lane = li_lane();
   int64_t total, share;
   balanced_share(a, waves, total, share);
@@ -527,11 +670,11 @@ __device__ __forceinline__ void decode_balanced_wave(const AttnArgs& a, int w, i
           int4{w, (int)((off + ctx - 1) / share), first_segment ? 0 : 1, 0};
     }
     const int row = decode_row(a, seq);
-    DecodeQuery<T, D, F8> q;
+    DecodeQuery<T, D, KV> q;
     load_query(a, row, kvh, q);
     DecodeState st;
     reset_state(st);
-    fold_keys<T, D, F8>(a, lds, q, seq, kvh, key0, key0 + take, st);
+    fold_keys<T, D, KV>(a, lds, q, seq, kvh, key0, key0 + take, st);
     if (key0 == 0 && take == ctx) {
       store_state<T, D>(st, static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)kvh * G * a.o_s1, a.o_s1,
                         nullptr, nullptr, 0, G, vscale);

@@ -129,6 +129,51 @@ __device__ __forceinline__ Frag lds_read_f8_vt(uint32_t addr) {
   return f8x8_to_frag<Frag>((uint32_t)v[0], (uint32_t)v[1]);
 }
 
+// What a pool holds: rows of the query's 16-bit type, fp8 (e4m3), or int8
+// codes with a scale for every (block, KV head). (false / true of the
+// kernels' pool argument are the first two.)
+constexpr int kPool16 = 0, kPoolF8 = 1, kPoolI8 = 2;
+
+// The 32-key tile of an int8 pool at head_dim 128: F8Tile, whose rows are as
+// many bytes. At head_dim 64 rows are 64 bytes (4 chunks of 16), four to a
+// 256-byte bank row, instruction i, row-in-instruction rr holding key 2 rr +
+// i; keys k, k + 1 (k even), k + 8 and k + 9 share a bank quarter, so the K
+// swizzle makes those four differ (16 keys of one chunk) and the V swizzle k,
+// k + 1, k + 16 and k + 17 (a transposing read's keys kappa(g, .)).
+struct I8Tile64 {
+  static constexpr int kCh = 4;
+  static constexpr int kRowsPerInst = 16;
+  static constexpr int kInsts = 2;
+  static constexpr int kRowBytes = 64;
+  static constexpr int kTileBytes = 2 * 32 * kRowBytes;  // K then V
+  static constexpr int kRow16 = (16 / kInsts) * kRowBytes;
+  __device__ static int row_of(int key) { return kRowsPerInst * (key % kInsts) + key / kInsts; }
+  __device__ static int kswizzle(int key) { return (key & 1) | (((key >> 3) & 1) << 1); }
+  __device__ static int vswizzle(int key) { return (key & 1) | (((key >> 4) & 1) << 1); }
+  __device__ static int offset(int key, int chunk) { return row_of(key) * kRowBytes + 16 * (chunk ^ kswizzle(key)); }
+  __device__ static int voffset(int key, int chunk) { return row_of(key) * kRowBytes + 16 * (chunk ^ vswizzle(key)); }
+};
+
+// Eight codes (bytes 0..7 of lo, hi) as a bf16 MFMA operand. A code fits
+// bf16's eight significant bits, so cutting its fp32 form short is exact.
+__device__ __forceinline__ bf16x8_t i8x8_to_bf16(uint32_t lo, uint32_t hi) {
+  u32x4_t w;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t x = (u < 2 ? lo : hi) >> (16 * (u & 1));
+    const uint32_t a = __float_as_uint((float)(int)(int8_t)x), b = __float_as_uint((float)(int)(int8_t)(x >> 8));
+    w[u] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  }
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+
+// The V^T operand of an int8 tile: one 8-bit transposing read at `addr`.
+__device__ __forceinline__ bf16x8_t lds_read_i8_vt(uint32_t addr) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  const v2i v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)addr);
+  return i8x8_to_bf16((uint32_t)v[0], (uint32_t)v[1]);
+}
+
 // One direct-to-LDS load: every lane's 16 bytes at `g` land at lds + 16 * lane.
 //
 // Written as inline assembly on purpose: the compiler models the builtin's

@@ -573,6 +573,27 @@ extern "C" int li_prefill_row_groups(unsigned long long row_keys, unsigned long 
                             num_heads, head_dim, kv_fp8);
 }
 
+// The workspace of an int8 pool's MFMA pass: what the 16-bit pass takes, then
+// the chunks' contexts in the query's dtype (byte offsets) and the table that
+// names their rows.
+struct ContextCopy {
+  int64_t rows = 0;
+  size_t table = 0, keys = 0, values = 0, need = 0;
+};
+ContextCopy context_copy(int batch, int num_heads, int num_kv_heads, int head_dim, int max_context, int max_query_len,
+                         int64_t context_tokens) {
+  ContextCopy c;
+  const int64_t most = std::max<int64_t>((int64_t)batch * max_context, 1);
+  c.rows = max_query_len <= 1 ? 0 : context_tokens > 0 ? std::min(context_tokens, most) : most;
+  const size_t bytes = align256((size_t)c.rows * num_kv_heads * head_dim * 2);
+  c.table = align256(prefill_workspace(balanced_waves(device_cu_count()), num_heads / num_kv_heads, head_dim, batch,
+                                       num_kv_heads, max_context));
+  c.keys = c.table + (c.rows ? align256((size_t)batch * std::max(max_context, 1) * sizeof(int64_t)) : 0);
+  c.values = c.keys + bytes;
+  c.need = c.values + bytes;
+  return c;
+}
+
 int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* key_pool,
                        const void* value_pool, int64_t pool_stride_slot, int64_t pool_stride_head,
                        const int64_t* slot_table, int64_t slot_table_stride, int max_context,
@@ -580,7 +601,7 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
                        void* out, int64_t out_stride_tok, int64_t out_stride_head, int num_heads, int num_kv_heads,
                        int head_dim, float scale, int block_q, int block_kv, void* workspace, size_t workspace_bytes,
                        int dtype, int kv_dtype, float k_scale, float v_scale, int flags, void* stream,
-                       const BlockScales* scales = nullptr) {
+                       const BlockScales* scales = nullptr, int64_t context_tokens = 0) {
   clear_error();
   if (int rc = check_common(dtype, num_heads, num_kv_heads, head_dim, "li_paged_prefill")) return rc;
   if (int rc = check_kv(dtype, kv_dtype, k_scale, v_scale, "li_paged_prefill")) return rc;
@@ -623,7 +644,37 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
   if (scales) set_block_scales(a, *scales);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool mfma = !(flags & LI_FLAG_FORCE_GENERIC) && prefill_mfma_applies(a, dtype);
+  // An int8 pool's one-query rows read the codes; its chunks read a copy of
+  // their contexts in the query's dtype.
+  const AttnArgs rows_of = a;
+  ContextCopy copy;
+  bool mfma = !(flags & LI_FLAG_FORCE_GENERIC);
+  // (A pass of single queries is a decode step: no copy.)
+  if (scales && max_query_len <= 1) flags &= ~LI_FLAG_PREFILL_ONLY;
+  if (scales && mfma) {
+    mfma = decode_mfma_applies(a, dtype) && copy_contexts_applies(a);
+    if (mfma) {
+      copy = context_copy(batch, num_heads, num_kv_heads, head_dim, max_context, max_query_len, context_tokens);
+      if (copy.rows >= (int64_t)1 << 31)
+        return fail(LI_EUNSUPPORTED, "li_paged_prefill_int8: contexts of %lld tokens are too many", (long long)copy.rows);
+      if (!workspace || workspace_bytes < copy.need)
+        return fail(LI_EWORKSPACE, "li_paged_prefill_int8: workspace of %zu bytes given, %zu needed", workspace_bytes,
+                    copy.need);
+      char* wp = static_cast<char*>(workspace);
+      a.kp = wp + copy.keys;
+      a.vp = wp + copy.values;
+      a.st = reinterpret_cast<int64_t*>(wp + copy.table);
+      a.st_s = max_context;
+      a.p_s0 = (int64_t)num_kv_heads * head_dim;
+      a.p_s1 = head_dim;
+    }
+  }
+  mfma = mfma && prefill_mfma_applies(a, dtype);
+  auto lay_out = [&](bool rows_elsewhere) -> int {
+    if (!scales) return LI_OK;
+    return launch_copy_contexts(rows_of, dtype, rows_elsewhere, copy.rows, const_cast<void*>(a.kp),
+                                const_cast<void*>(a.vp), const_cast<int64_t*>(a.st), s);
+  };
   if (a.kv_fp8 && !mfma)
     return fail(LI_EUNSUPPORTED,
                 "li_paged_prefill: fp8 pools run on the MFMA kernels only (bf16 / fp16 queries, head_dim 128, "
@@ -661,8 +712,17 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
       wp += align256((size_t)prefill_grid() * kPrefillUnitRows * 2 * sizeof(float));
       a.split_first = reinterpret_cast<int*>(wp);
     }
-    if (flags & LI_FLAG_PREFILL_ONLY) return launch_prefill_mfma(a, dtype, s);
+    if (flags & LI_FLAG_PREFILL_ONLY) {
+      if (int rc = lay_out(false)) return rc;
+      return launch_prefill_mfma(a, dtype, s);
+    }
     AttnArgs d = a;
+    d.kp = rows_of.kp;
+    d.vp = rows_of.vp;
+    d.p_s0 = rows_of.p_s0;
+    d.p_s1 = rows_of.p_s1;
+    d.st = rows_of.st;
+    d.st_s = rows_of.st_s;
     d.block_q = 1;
     d.num_qblocks = 1;
     set_balanced(d, waves, workspace);
@@ -671,6 +731,7 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
       // per-head split, which fits the prefill kernels' registers.
       d.part_heads = 1;
       d.num_parts = waves;
+      if (int rc = lay_out(true)) return rc;
       return launch_prefill_with_rows(a, d, dtype, s);
     }
     if (int rc = launch_decode_mfma(d, dtype, s)) return rc;
@@ -679,6 +740,7 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
     return launch_prefill_mfma(a, dtype, s);
   }
   if (!(flags & LI_FLAG_FORCE_GENERIC) && attend_f32_applies(a, dtype)) return launch_attend_f32(a, s);
+  a = rows_of;
   a.block_q = block_q > 0 ? block_q : 16;
   a.num_qblocks = cdiv(max_query_len, a.block_q);
   return launch_attend_generic(a, dtype, s);
@@ -721,7 +783,13 @@ extern "C" int li_paged_prefill_int8_plan(int batch, int num_heads, int num_kv_h
   if (int rc = check_common(dtype, num_heads, num_kv_heads, head_dim, "li_paged_prefill_int8_plan")) return rc;
   if (batch < 0 || max_context < 0 || max_query_len < 0 || context_tokens < 0)
     return fail(LI_EINVAL, "li_paged_prefill_int8_plan: negative extent");
-  if (workspace_bytes) *workspace_bytes = 0;
+  // Shapes that the MFMA kernels do not serve need none.
+  const int groups = num_heads / num_kv_heads;
+  const bool mfma = (dtype == LI_BF16 || dtype == LI_F16) && (head_dim == 64 || head_dim == 128) && groups <= 16;
+  if (workspace_bytes)
+    *workspace_bytes =
+        mfma ? context_copy(batch, num_heads, num_kv_heads, head_dim, max_context, max_query_len, context_tokens).need
+             : 0;
   return LI_OK;
 }
 
@@ -741,5 +809,5 @@ extern "C" int li_paged_prefill_int8(const void* q, int64_t q_stride_tok, int64_
                             slot_table, slot_table_stride, max_context, context_lens, query_start_loc, batch,
                             max_query_len, out, out_stride_tok, out_stride_head, num_heads, num_kv_heads, head_dim,
                             scale, block_q, block_kv, workspace, workspace_bytes, dtype, dtype, 1.f, 1.f, flags,
-                            stream, &scales);
+                            stream, &scales, context_tokens);
 }

@@ -142,7 +142,7 @@ __device__ __forceinline__ void convert_stage(uint32_t raw, uint32_t dst, int ti
 // flight per wave, measured no faster: config 3 flat at 310-315 us from 48
 // row work-groups.)
 
-template <typename T, int D, bool F8, typename Shared>
+template <typename T, int D, int KV, typename Shared>
 __device__ __forceinline__ void fold_rows_first(const AttnArgs& a, const AttnArgs& d, Shared& lds) {
   // prefill_order's count (prefill_row_groups, at most a.row_groups_max,
   // which the host holds to the grid and to the workspace's partial slots),
@@ -165,7 +165,7 @@ __device__ __forceinline__ void fold_rows_first(const AttnArgs& a, const AttnArg
         const int per_head = waves / d.num_kv_heads;
         v = ((wg / per_head) * kRowWaves + rw) * per_head + wg % per_head;
       }
-      decode_balanced_wave<T, D, F8>(d, v, (int64_t)waves, lds.rows[rw]);
+      decode_balanced_wave<T, D, KV>(d, v, (int64_t)waves, lds.rows[rw]);
     }
     // (Every row wave's loads have landed: its folds consumed them.)
     __syncthreads();
@@ -758,22 +758,23 @@ struct PpLds {
 
 
 // LDS of a ping-pong work-group; prefill_pp_rows's row waves use it first.
-template <int D>
+template <int D, int KVR>
 union PpShared {
   PpLds<D> pp;
-  DecodeLds<D, false> rows[kRowWaves];
+  DecodeLds<D, KVR> rows[kRowWaves];
 };
 
 // The ping-pong work of work-group blockIdx.x of the persistent grid (its
 // queue: blockIdx.x % kPrefillQueues). With kRows (prefill_pp_rows), the
 // first work-groups fold the pass's one-query rows first (the balanced
 // decode split, AttnArgs `d`, over kRowWaves waves of each of them; their
-// count was written by prefill_order), then join the queues.
-template <typename T, int D, bool kRows, bool kSplit, bool kDirect = false>
+// count was written by prefill_order), then join the queues. KVR: what the
+// rows' pool holds (int8 codes, or the type of the pool that the chunks read).
+template <typename T, int D, bool kRows, bool kSplit, bool kDirect = false, int KVR = kPool16>
 __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
-  __shared__ __attribute__((aligned(1024))) PpShared<D> lds;
+  __shared__ __attribute__((aligned(1024))) PpShared<D, KVR> lds;
   const unsigned wg = blockIdx.x;
-  if constexpr (kRows) fold_rows_first<T, D, false>(a, d, lds);
+  if constexpr (kRows) fold_rows_first<T, D, KVR>(a, d, lds);
   constexpr int W = 8;
   using M = Mfma<T>;
   using Frag = typename M::Frag;
@@ -1357,10 +1358,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // each), while the others start on the chunks; each joins the chunks'
 // queues when its rows are done. The rows stream K/V from HBM while the
 // chunks keep the matrix cores busy, instead of one waiting for the other.
-template <typename T, int D, bool kSplit>
+template <typename T, int D, bool kSplit, int KVR>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_pp_rows(AttnArgs a,
                                                                                                   AttnArgs d) {
-  prefill_pp_body<T, D, true, kSplit>(a, d);
+  prefill_pp_body<T, D, true, kSplit, false, KVR>(a, d);
 }
 
 // Work list of the prefill grid: every non-empty query block
@@ -1552,7 +1553,7 @@ __global__ __launch_bounds__(1024) void prefill_order(AttnArgs a) {
     __syncthreads();
     if (tid == 0)
       a.queue[kPrefillQueues + 1] = prefill_row_groups(row_keys, chunk_pairs, max_tiles, a.row_groups_max,
-                                                       a.num_kv_heads, a.num_heads, a.head_dim, a.kv_fp8);
+                                                       a.num_kv_heads, a.num_heads, a.head_dim, a.kv_fp8 | a.kv_int8);
   }
 }
 
@@ -1664,7 +1665,6 @@ bool prefill_mfma_applies(const AttnArgs& a, int dtype) {
   if (dtype != LI_BF16 && dtype != LI_F16) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.kv_fp8 && a.head_dim != 128) return false;
-  if (a.kv_int8) return false;
   if (a.groups < 1 || a.groups > 16) return false;
   const int pe = a.kv_fp8 ? 1 : 2;
   return rows_aligned(a.q, a.q_s0, a.q_s1, 2) && rows_aligned(a.out, a.o_s0, a.o_s1, 2) &&
@@ -1725,10 +1725,15 @@ static int launch_prefill_waves(AttnArgs a, int dtype, hipStream_t s, const Attn
     return launch_combine_balanced(*rows, dtype, s);
   }
   if (rows) {
-#define LI_PP_ROWS(T, D)                                                                            \
-  do {                                                                                              \
-    if (a.split_ok) hipLaunchKernelGGL((prefill_pp_rows<T, D, true>), g, block, 0, s, a, *rows);    \
-    else hipLaunchKernelGGL((prefill_pp_rows<T, D, false>), g, block, 0, s, a, *rows);              \
+#define LI_PP_ROWS_OF(T, D, KVR)                                                                       \
+  do {                                                                                                 \
+    if (a.split_ok) hipLaunchKernelGGL((prefill_pp_rows<T, D, true, KVR>), g, block, 0, s, a, *rows);  \
+    else hipLaunchKernelGGL((prefill_pp_rows<T, D, false, KVR>), g, block, 0, s, a, *rows);            \
+  } while (0)
+#define LI_PP_ROWS(T, D)                                  \
+  do {                                                    \
+    if (rows->kv_int8) LI_PP_ROWS_OF(T, D, kPoolI8);      \
+    else LI_PP_ROWS_OF(T, D, kPool16);                    \
   } while (0)
     if (dtype == LI_BF16) {
       if (a.head_dim == 128) LI_PP_ROWS(li_bf16, 128);
@@ -1738,6 +1743,7 @@ static int launch_prefill_waves(AttnArgs a, int dtype, hipStream_t s, const Attn
       else LI_PP_ROWS(li_f16, 64);
     }
 #undef LI_PP_ROWS
+#undef LI_PP_ROWS_OF
     if (int rc = check_launch("prefill_pp_rows")) return rc;
     if (int rc = launch_prefill_merge(a, dtype, s, false)) return rc;
     return launch_combine_balanced(*rows, dtype, s);
