@@ -544,6 +544,36 @@ int li_silu_mul_partials(const float* partials, int splits, void* out,
                          void* stream);
 
 /*
+ * The engine's projections in 8-bit integers: out = x w^T for x [m, k] of
+ * dtype (LI_F32, LI_F16 or LI_BF16, last axis contiguous) and w [n, k] int8
+ * codes, whose row j stands for code * w_scales[j]. x is quantised on the way
+ * in, row by row:
+ *     scale = max(largest magnitude / 127, 2^-126), code = rint(x / scale)
+ * in fp32 (the quotient as a product with 1 / scale), the products are summed
+ * exactly in int32 (k <= LI_INT8_MAX_K) and
+ *     out[i, j] = sum * scale[i] * w_scales[j]
+ * is rounded once. A row of x with a value that is not finite gives NaN.
+ * w's rows start at multiples of 16 bytes (w and w_stride) and are readable up
+ * to the next multiple of 16 past k, whatever lies there. The workspace holds
+ * what li_linear_int8_plan reports (x's codes and scales, and the sums of the
+ * runs that k may be cut into). No counterpart in the reference, whose
+ * projections are nn.Linear (liteinfer/models/llama.py:101-161).
+ *
+ * li_quantize_rows: the codes and scales of x by themselves (and, by the same
+ * rule, those of a weight): codes [rows, padded] with zeros from k on, rows
+ * codes_stride apart, 8-byte aligned.
+ */
+#define LI_INT8_MAX_K 131072
+int li_quantize_rows(const void* x, int64_t x_stride, void* codes,
+                     int64_t codes_stride, float* scales, int rows, int k,
+                     int padded, int dtype, void* stream);
+int li_linear_int8_plan(int m, int n, int k, size_t* workspace_bytes);
+int li_linear_int8(const void* x, int64_t x_stride, const void* w,
+                   int64_t w_stride, const float* w_scales, void* out,
+                   int64_t out_stride, int m, int n, int k, void* workspace,
+                   size_t workspace_bytes, int dtype, void* stream);
+
+/*
  * The engine's per-step inputs, one launch each (chains of torch copies and
  * elementwise ops otherwise).
  *

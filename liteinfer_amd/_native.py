@@ -67,6 +67,9 @@ EXPORTED_SYMBOLS = (
     "li_skinny_reduce",
     "li_add_rms_norm_partials",
     "li_silu_mul_partials",
+    "li_quantize_rows",
+    "li_linear_int8_plan",
+    "li_linear_int8",
     "li_rotary_tables",
     "li_stage_decode",
 )
@@ -82,6 +85,9 @@ _SIGNATURES = {
     "li_skinny_reduce": (_i32, [_p, _p, _i64, _i32, _i32, _i32, _i32, _p]),
     "li_add_rms_norm_partials": (_i32, [_p, _p, _i32, _p, _p, _i64, _i32, _i64, _i64, _f32, _i32, _p]),
     "li_silu_mul_partials": (_i32, [_p, _i32, _p, _i64, _i32, _i64, _i32, _p]),
+    "li_quantize_rows": (_i32, [_p, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32, _p]),
+    "li_linear_int8_plan": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_sz)]),
+    "li_linear_int8": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _p, _sz, _i32, _p]),
     "li_rotary_tables": (_i32, [_p, _p, _p, _p, _i64, _i32, _i32, _p]),
     "li_stage_decode": (_i32, [_p, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _i64, _p, _i32, _i32, _i32, _i64, _p]),
     "li_last_error_string": (ctypes.c_char_p, []),

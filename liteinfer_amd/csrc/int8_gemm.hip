@@ -1,0 +1,447 @@
+// out = x w^T in 8-bit integers: x [m, k] quantised on the way in with a scale
+// for each row (token), w [n, k] held as codes with a scale for each of its
+// rows (output channel).
+//     sx[i]  = max(largest |x[i, :]| / 127, 2^-126)
+//     c[i]   = rint(x[i, :] / sx[i])              (as a product with 1 / sx[i])
+//     out[i, j] = (sum_k c[i, k] w[j, k]) * sx[i] * sw[j]
+// The sums are int32 and exact (k <= LI_INT8_MAX_K keeps 127^2 k below 2^31);
+// scales and their products are fp32, the output is rounded once. A row that
+// holds a value that is not finite gets a NaN scale, so its outputs are NaN.
+//
+// Everything moves in bytes as a 16-bit product of half the k would: an
+// operand of v_mfma_i32_16x16x64_i8 is 16 codes (16 bytes) a lane, lane
+// (r, g) = (lane % 16, lane / 16) holding bytes 16 g .. of 64 of row r.
+// Operand A is 16 rows of w, B 16 rows of x, so lane (r, g) ends with outputs
+// 4 g .. 4 g + 3 of row r: four neighbours in memory.
+//
+// Codes past k are zero in x (its codes are laid out in rows of a multiple
+// of kPadK), so whatever is read of w there does not count; reads of w are
+// held to its rows' last 16 bytes.
+#include "li_mfma.h"
+
+namespace {
+
+using namespace li;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr int kPadK = 256;
+constexpr float kStep = 1.0f / 127.0f;
+constexpr float kLeast = 1.17549435e-38f;  // 2^-126
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+template <typename E>
+using Vec8 = __attribute__((__vector_size__(8 * sizeof(E)), __aligned__(16))) E;
+
+// A row's scale (as bits) and its codes' factor, from the bits of its largest
+// magnitude (which order what is not finite above the rest).
+struct RowScale {
+  uint32_t bits;
+  float inv;  // 0: not finite, every code 0
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t largest) {
+  const bool lost = largest >= kInfBits;
+  const float s = fmaxf(__uint_as_float(lost ? 0u : largest) * kStep, kLeast);
+  return {lost ? 0x7fc00000u : __float_as_uint(s), lost ? 0.f : 1.f / s};
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+  return (uint32_t)(int)fminf(fmaxf(rintf(x * inv), -127.f), 127.f) & 255u;
+}
+
+template <typename E>
+__device__ __forceinline__ uint2 codes_of(const Vec8<E>& x, float inv, bool lost) {
+  uint32_t w[2] = {0u, 0u};
+  if (!lost) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e / 4] |= code_of(li_to_float(x[e]), inv) << (8 * (e % 4));
+  }
+  return uint2{w[0], w[1]};
+}
+
+template <typename E>
+__device__ __forceinline__ uint32_t largest_of(const Vec8<E>& x) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(li_to_float(x[e])) & 0x7fffffffu);
+  return top;
+}
+
+// ---------------------------------------------------------------------------
+// Quantising rows: one work-group a row. Up to kHold x 2,048 values stay in
+// registers between the maximum and the codes; longer rows are read twice.
+// Memory-bound.
+// ---------------------------------------------------------------------------
+constexpr int kQuantThreads = 256;
+
+// Eight values of a row from column d (zeros past k), whatever its alignment.
+template <typename E, bool kVec>
+__device__ __forceinline__ Vec8<E> row_values(const E* row, int d, int k) {
+  if constexpr (kVec) {
+    if (d + 8 <= k) return *reinterpret_cast<const Vec8<E>*>(row + d);
+  }
+  Vec8<E> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = d + e < k ? row[d + e] : li_from_float<E>(0.f);
+  return v;
+}
+
+template <typename E, bool kVec>
+__global__ __launch_bounds__(kQuantThreads) void quantize_rows(const E* x, int64_t x_s, int8_t* codes, int64_t c_s,
+                                                               float* scales, int k, int padded) {
+  constexpr int kHold = 8;
+  const int tid = threadIdx.x;
+  const E* row = x + (int64_t)blockIdx.x * x_s;
+  Vec8<E> held[kHold];
+  uint32_t top = 0;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int d = 8 * (tid + kQuantThreads * u);
+    if (d < k) {
+      held[u] = row_values<E, kVec>(row, d, k);
+      top = max(top, largest_of<E>(held[u]));
+    }
+  }
+  for (int d = 8 * (tid + kQuantThreads * kHold); d < k; d += 8 * kQuantThreads)
+    top = max(top, largest_of<E>(row_values<E, kVec>(row, d, k)));
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  __shared__ uint32_t tops[kQuantThreads / 64];
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQuantThreads / 64; ++w) top = max(top, tops[w]);
+  const RowScale s = row_scale(top);
+  const bool lost = top >= kInfBits;
+  int8_t* out = codes + (int64_t)blockIdx.x * c_s;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int d = 8 * (tid + kQuantThreads * u);
+    if (d < k) *reinterpret_cast<uint2*>(out + d) = codes_of<E>(held[u], s.inv, lost);
+    else if (d < padded) *reinterpret_cast<uint2*>(out + d) = uint2{0u, 0u};
+  }
+  for (int d = 8 * (tid + kQuantThreads * kHold); d < padded; d += 8 * kQuantThreads)
+    *reinterpret_cast<uint2*>(out + d) = d < k ? codes_of<E>(row_values<E, kVec>(row, d, k), s.inv, lost) : uint2{0u, 0u};
+  if (tid == 0) reinterpret_cast<uint32_t*>(scales)[blockIdx.x] = s.bits;
+}
+
+// ---------------------------------------------------------------------------
+// The product.
+// ---------------------------------------------------------------------------
+
+struct GemmArgs {
+  const char* x;     // codes [m, x_s], zero from k to a multiple of kPadK
+  const float* xs;   // [m]
+  const char* w;     // codes [n, w_s]
+  const float* ws;   // [n]
+  char* out;         // T rows (splits == 1)
+  int32_t* part;     // [splits][m][n] sums (splits > 1)
+  int64_t x_s, w_s;  // row strides in bytes
+  int64_t o_s;       // out: in elements
+  int m, n, k;
+  int splits;
+  int vec;           // four outputs side by side may be stored at once
+  int mt, nt;        // tiles of rows of x, of w
+};
+
+// Four sums for outputs n .. n + 3 of row m.
+template <typename T>
+__device__ __forceinline__ void store4(const GemmArgs& a, const v4i& acc, int split, int m, int n) {
+  if (m >= a.m || n >= a.n) return;
+  if (a.splits > 1) {
+    int32_t* p = a.part + ((int64_t)split * a.m + m) * a.n + n;
+    if (a.vec && n + 4 <= a.n) {
+      *reinterpret_cast<v4i*>(p) = acc;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.n) p[r] = acc[r];
+    }
+    return;
+  }
+  const float sx = a.xs[m];
+  T* o = reinterpret_cast<T*>(a.out) + m * a.o_s + n;
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = n + r < a.n ? (float)acc[r] * sx * a.ws[n + r] : 0.f;
+  if (a.vec && n + 4 <= a.n) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<floatx4_t*>(o) = floatx4_t{v[0], v[1], v[2], v[3]};
+    else *reinterpret_cast<uint2*>(o) = uint2{li_pack2<T>(v[0], v[1]), li_pack2<T>(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < a.n) o[r] = li_from_float<T>(v[r]);
+  }
+}
+
+// Waits until at most `newer` stages of kPer loads each are in flight.
+template <int R, int kPer>
+__device__ __forceinline__ void wait_stages(int newer) {
+  static_assert(R >= 2 && R <= 8 && (R - 2) * kPer < 64, "vmcnt range");
+  if (R > 7 && newer >= 6) li_wait_vm<(R > 7 ? 6 * kPer : 0)>();
+  else if (R > 6 && newer >= 5) li_wait_vm<(R > 6 ? 5 * kPer : 0)>();
+  else if (R > 5 && newer >= 4) li_wait_vm<(R > 5 ? 4 * kPer : 0)>();
+  else if (R > 4 && newer >= 3) li_wait_vm<(R > 4 ? 3 * kPer : 0)>();
+  else if (R > 3 && newer >= 2) li_wait_vm<(R > 3 ? 2 * kPer : 0)>();
+  else if (R > 2 && newer >= 1) li_wait_vm<(R > 2 ? kPer : 0)>();
+  else li_wait_vm<0>();
+}
+
+// A work-group of WM x WN waves takes BM rows of x by BN rows of w and a run
+// of k, both operands straight into LDS in a ring of R stages of RB bytes a
+// row: chunk c (16 bytes) of row r at c ^ (r / (256 / RB)) % (RB / 16), so that
+// the 16 rows an operand read spans lie in 16 different bank groups. R - 1
+// stages are in flight, one barrier a stage.
+template <typename T, int BM, int BN, int WM, int WN, int RB, int R>
+__global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
+  constexpr int kWaves = WM * WN;
+  constexpr int kCh = RB / 16, kQ = 256 / RB;  // chunks of a row, rows of a 256-byte bank row
+  constexpr int kRows = 64 / kCh;              // rows one load fills
+  constexpr int kLoads = (BM + BN) / kRows, kPer = kLoads / kWaves;
+  static_assert(kPer >= 1 && kPer * kWaves == kLoads, "the waves split a stage's loads evenly");
+  constexpr int kFm = BM / WM / 16, kFn = BN / WN / 16, kK = RB / 64;
+  constexpr int kStage = (BM + BN) * RB;
+  __shared__ __attribute__((aligned(1024))) char ring[R][kStage];
+  const int lane = (int)(threadIdx.x & 63);
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int r16 = lane & 15, g = lane >> 4;
+
+  // Work-group i runs on XCD i % 8; each XCD takes a run of tiles, side by
+  // side along x's rows first, so that its L2 serves a tile of w to several.
+  const int total = a.mt * a.nt * a.splits;
+  const int per = total / 8, rest = total % 8;
+  const int xcd = (int)(blockIdx.x % 8u), at = (int)(blockIdx.x / 8u);
+  const int t = xcd * per + min(xcd, rest) + at;
+  const int split = t % a.splits, tile = t / a.splits;
+  const int tm = tile % a.mt, tn = tile / a.mt;
+  const int stages = (a.k + RB - 1) / RB;
+  const int s0 = (int)((int64_t)stages * split / a.splits), s1 = (int)((int64_t)stages * (split + 1) / a.splits);
+  const int ns = s1 - s0;
+
+  // Load i of this wave fills rows kRows * (wv * kPer + i) .. of the stage
+  // (x's rows first); a lane brings one chunk. Rows past the last repeat it.
+  const char* src[kPer];
+  int col[kPer], cap[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int row = kRows * (wv * kPer + i) + lane / kCh;
+    col[i] = 16 * ((lane % kCh) ^ ((row / kQ) % kCh)) + s0 * RB;
+    src[i] = row < BM ? a.x + (int64_t)min(tm * BM + row, a.m - 1) * a.x_s
+                      : a.w + (int64_t)min(tn * BN + row - BM, a.n - 1) * a.w_s;
+    // w's rows end at their last chunk; x's go on in zeros.
+    cap[i] = row < BM ? 0x7fffffff : (a.k + 15) / 16 * 16 - 16;
+  }
+  const uint32_t base = lds_addr(&ring[0][0]);
+  auto issue = [&](int st) {
+    const uint32_t dst = base + (uint32_t)(st % R) * kStage + (uint32_t)wv * kPer * 1024;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) dma16<false>(src[i] + min(col[i] + st * RB, cap[i]), dst + 1024 * i);
+  };
+
+  v4i acc[kFm][kFn];
+#pragma unroll
+  for (int i = 0; i < kFm; ++i)
+#pragma unroll
+    for (int j = 0; j < kFn; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  const int wm = wv % WM, wn = wv / WM;
+  uint32_t off[kK];
+#pragma unroll
+  for (int j = 0; j < kK; ++j) off[j] = (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ ((r16 / kQ) % kCh)));
+
+#pragma unroll
+  for (int st = 0; st < R - 1; ++st)
+    if (st < ns) issue(st);
+  for (int st = 0; st < ns; ++st) {
+    wait_stages<R, kPer>(min(R - 2, ns - 1 - st));
+    lds_barrier();  // every wave's part of it; and all are done with stage st - 1, whose place the next loads take
+    if (st + R - 1 < ns) issue(st + R - 1);
+    const uint32_t xc = base + (uint32_t)(st % R) * kStage + (uint32_t)wm * (BM / WM) * RB;
+    const uint32_t wc = base + (uint32_t)(st % R) * kStage + (uint32_t)(BM + wn * (BN / WN)) * RB;
+#pragma unroll
+    for (int j = 0; j < kK; ++j) {
+      v4i xf[kFm], wf[kFn];
+#pragma unroll
+      for (int f = 0; f < kFn; ++f) wf[f] = lds_read_frag<v4i>(wc + f * 16 * RB + off[j]);
+#pragma unroll
+      for (int i = 0; i < kFm; ++i) xf[i] = lds_read_frag<v4i>(xc + i * 16 * RB + off[j]);
+#pragma unroll
+      for (int i = 0; i < kFm; ++i)
+#pragma unroll
+        for (int f = 0; f < kFn; ++f) acc[i][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f], xf[i], acc[i][f], 0, 0, 0);
+    }
+    // The stage's reads are complete before the next stage's barrier is reached.
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int i = 0; i < kFm; ++i)
+#pragma unroll
+    for (int f = 0; f < kFn; ++f)
+      store4<T>(a, acc[i][f], split, tm * BM + wm * (BM / WM) + 16 * i + r16, tn * BN + wn * (BN / WN) + 16 * f + 4 * g);
+}
+
+// out = the splits' sums, scaled and rounded.
+template <typename T>
+__global__ __launch_bounds__(256) void reduce_sums(GemmArgs a) {
+  const int64_t quads = (a.n + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.m * quads) return;
+  const int m = (int)(i / quads), n = (int)(i - m * quads) * 4;
+  v4i s = {0, 0, 0, 0};
+  for (int p = 0; p < a.splits; ++p) {
+    const int32_t* src = a.part + ((int64_t)p * a.m + m) * a.n + n;
+    if (a.vec && n + 4 <= a.n) {
+      s += *reinterpret_cast<const v4i*>(src);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.n) s[r] += src[r];
+    }
+  }
+  GemmArgs whole = a;
+  whole.splits = 1;
+  store4<T>(whole, s, 0, m, n);
+}
+
+// Which kernel a product runs on and the runs its k is cut into.
+enum Kind { kFew, kSome, kMany, kMost };
+struct Plan {
+  Kind kind;
+  int bm, bn, splits;
+};
+Plan plan_of(int m, int n, int k) {
+  const int cus = li::device_cu_count();
+  Plan p{};
+  if (m <= 16) p = {kFew, 16, 64, 1};
+  else if (m <= 64) p = {kSome, 64, 64, 1};
+  else if ((int64_t)cdiv(m, 256) * cdiv(n, 256) < cus) p = {kMany, 128, 128, 1};
+  else p = {kMost, 256, 256, 1};
+  const int64_t tiles = (int64_t)cdiv(m, p.bm) * cdiv(n, p.bn);
+  if (tiles * 4 < cus * 3) p.splits = std::max<int>(1, std::min<int64_t>(cus / tiles, cdiv(k, 1024)));
+  return p;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct Space {
+  int64_t x_s;
+  size_t scales, part, need;  // byte offsets: the codes come first
+};
+Space space_of(int m, int n, int k) {
+  Space s;
+  const Plan p = plan_of(m, n, k);
+  s.x_s = (int64_t)(k + kPadK - 1) / kPadK * kPadK;
+  s.scales = align256((size_t)m * s.x_s);
+  s.part = s.scales + align256((size_t)m * sizeof(float));
+  s.need = s.part + (p.splits > 1 ? align256((size_t)p.splits * m * n * sizeof(int32_t)) : 0);
+  return s;
+}
+
+int check_extents(const char* who, int m, int n, int k) {
+  if (m < 0 || n <= 0 || k <= 0) return li::fail(LI_EINVAL, "%s: bad extents (%d, %d, %d)", who, m, n, k);
+  if (k > LI_INT8_MAX_K)
+    return li::fail(LI_EUNSUPPORTED, "%s: sums of %d products pass 32 bits, %d at most", who, k, LI_INT8_MAX_K);
+  return LI_OK;
+}
+
+template <typename E>
+void launch_quantize(const void* x, int64_t x_s, void* codes, int64_t c_s, float* scales, int m, int k, int padded,
+                     hipStream_t s) {
+  const bool vec = li::aligned16(x) && (x_s * (int64_t)sizeof(E)) % 16 == 0;
+  const E* xp = static_cast<const E*>(x);
+  int8_t* cp = static_cast<int8_t*>(codes);
+  if (vec) hipLaunchKernelGGL((quantize_rows<E, true>), dim3((unsigned)m), dim3(kQuantThreads), 0, s, xp, x_s, cp, c_s, scales, k, padded);
+  else hipLaunchKernelGGL((quantize_rows<E, false>), dim3((unsigned)m), dim3(kQuantThreads), 0, s, xp, x_s, cp, c_s, scales, k, padded);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int RB, int R>
+void launch_ring(GemmArgs a, hipStream_t s) {
+  a.mt = cdiv(a.m, BM);
+  a.nt = cdiv(a.n, BN);
+  const dim3 grid((unsigned)(a.mt * a.nt * a.splits)), block(64 * WM * WN);
+  hipLaunchKernelGGL((ring_gemm<T, BM, BN, WM, WN, RB, R>), grid, block, 0, s, a);
+}
+
+template <typename T>
+void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
+  switch (kind) {
+    case kFew: launch_ring<T, 16, 64, 1, 4, 256, 5>(a, s); break;
+    case kSome: launch_ring<T, 64, 64, 2, 2, 256, 4>(a, s); break;
+    case kMany: launch_ring<T, 128, 128, 2, 2, 128, 4>(a, s); break;
+    case kMost: launch_ring<T, 256, 256, 2, 4, 64, 4>(a, s); break;
+  }
+  if (a.splits > 1) {
+    const int64_t work = (int64_t)a.m * ((a.n + 3) / 4);
+    hipLaunchKernelGGL(reduce_sums<T>, dim3((unsigned)cdiv64(work, 256)), dim3(256), 0, s, a);
+  }
+}
+
+}  // namespace
+
+extern "C" int li_quantize_rows(const void* x, int64_t x_stride, void* codes, int64_t codes_stride, float* scales,
+                                int rows, int k, int padded, int dtype, void* stream) {
+  li::clear_error();
+  if (dtype != LI_F32 && dtype != LI_F16 && dtype != LI_BF16)
+    return li::fail(LI_EINVAL, "li_quantize_rows: unknown dtype %d", dtype);
+  if (rows < 0 || k <= 0 || padded < k || codes_stride < padded)
+    return li::fail(LI_EINVAL, "li_quantize_rows: bad extents (%d, %d, %d)", rows, k, padded);
+  if (rows == 0) return LI_OK;
+  if (!x || !codes || !scales) return li::fail(LI_EINVAL, "li_quantize_rows: null pointer");
+  if ((reinterpret_cast<uintptr_t>(codes) & 7) || codes_stride % 8 || padded % 8)
+    return li::fail(LI_EINVAL, "li_quantize_rows: rows of codes must be 8-byte aligned and padded");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == LI_F32) launch_quantize<float>(x, x_stride, codes, codes_stride, scales, rows, k, padded, s);
+  else if (dtype == LI_F16) launch_quantize<li_f16>(x, x_stride, codes, codes_stride, scales, rows, k, padded, s);
+  else launch_quantize<li_bf16>(x, x_stride, codes, codes_stride, scales, rows, k, padded, s);
+  return li::check_launch("li_quantize_rows");
+}
+
+extern "C" int li_linear_int8_plan(int m, int n, int k, size_t* workspace_bytes) {
+  li::clear_error();
+  if (int rc = check_extents("li_linear_int8_plan", m, n, k)) return rc;
+  if (workspace_bytes) *workspace_bytes = m ? space_of(m, n, k).need : 0;
+  return LI_OK;
+}
+
+extern "C" int li_linear_int8(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const float* w_scales,
+                              void* out, int64_t out_stride, int m, int n, int k, void* workspace,
+                              size_t workspace_bytes, int dtype, void* stream) {
+  li::clear_error();
+  const int esize = li::dtype_size(dtype);
+  if (dtype != LI_F32 && dtype != LI_F16 && dtype != LI_BF16)
+    return li::fail(LI_EINVAL, "li_linear_int8: unknown dtype %d", dtype);
+  if (int rc = check_extents("li_linear_int8", m, n, k)) return rc;
+  if (m == 0) return LI_OK;
+  if (!x || !w || !w_scales || !out) return li::fail(LI_EINVAL, "li_linear_int8: null pointer");
+  if (!li::aligned16(w) || w_stride % 16 || w_stride < (k + 15) / 16 * 16)
+    return li::fail(LI_EINVAL, "li_linear_int8: rows of w must start at multiples of 16 bytes and be padded to them");
+  if (out_stride < n || x_stride < 0) return li::fail(LI_EINVAL, "li_linear_int8: rows overlap");
+  const Plan p = plan_of(m, n, k);
+  const Space sp = space_of(m, n, k);
+  if (!workspace || !li::aligned16(workspace) || workspace_bytes < sp.need)
+    return li::fail(LI_EWORKSPACE, "li_linear_int8: workspace of %zu bytes given, %zu needed", workspace_bytes, sp.need);
+  if ((int64_t)cdiv(m, p.bm) * cdiv(n, p.bn) * p.splits > 0x7fffffffLL)
+    return li::fail(LI_EUNSUPPORTED, "li_linear_int8: %d x %d outputs are too many tiles", m, n);
+  char* wp = static_cast<char*>(workspace);
+  float* xs = reinterpret_cast<float*>(wp + sp.scales);
+  if (int rc = li_quantize_rows(x, x_stride, wp, sp.x_s, xs, m, k, (int)sp.x_s, dtype, stream)) return rc;
+  GemmArgs a{};
+  a.x = wp;
+  a.xs = xs;
+  a.w = static_cast<const char*>(w);
+  a.ws = w_scales;
+  a.out = static_cast<char*>(out);
+  a.part = reinterpret_cast<int32_t*>(wp + sp.part);
+  a.x_s = sp.x_s;
+  a.w_s = w_stride;
+  a.o_s = out_stride;
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.splits = p.splits;
+  a.vec = n % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == LI_F32) launch_gemm<float>(a, p.kind, s);
+  else if (dtype == LI_F16) launch_gemm<li_f16>(a, p.kind, s);
+  else launch_gemm<li_bf16>(a, p.kind, s);
+  return li::check_launch("li_linear_int8");
+}

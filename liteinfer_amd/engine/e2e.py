@@ -38,10 +38,11 @@ def prompts(seed: int = 0, n: int = NUM_REQUESTS, vocab: int = LLAMA_3_8B.vocab_
 
 
 def run(seed: int = 0, config: EngineConfig | None = None, num_requests: int = NUM_REQUESTS,
-        output_tokens: int = OUTPUT_TOKENS, cache_quant: str | None = None) -> dict:
+        output_tokens: int = OUTPUT_TOKENS, cache_quant: str | None = None,
+        weight_quant: str | None = None) -> dict:
     config = config or EngineConfig(max_num_seqs=256, max_model_len=PROMPT_CLIP[1] + OUTPUT_TOKENS,
                                     max_num_batched_tokens=8192, num_gpu_blocks=32768, cache_quant=cache_quant)
-    model = RandomLlama(LLAMA_3_8B, seed=seed)
+    model = RandomLlama(LLAMA_3_8B, seed=seed, weight_quant=weight_quant)
     with tempfile.TemporaryDirectory(prefix="liteinfer_amd_tok_") as tok_dir:
         make_wordlevel(model.shape.vocab_size, tok_dir)
         tokenizer = Tokenizer(tok_dir)
@@ -75,6 +76,7 @@ def run(seed: int = 0, config: EngineConfig | None = None, num_requests: int = N
         "max_num_batched_tokens": config.max_num_batched_tokens,
         "decode_graphs": config.use_graphs,
         "kv_cache": config.cache_quant or "bf16",
+        "projections": weight_quant or "bf16",
         "parameter_bytes": model.parameter_bytes(),
         # properties of the timed run's output, checked after the clock stops
         "every_request_full_length": all(len(o) == output_tokens for o in outputs),

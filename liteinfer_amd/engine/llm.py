@@ -34,7 +34,8 @@ class EngineConfig:
     block_size: int = 16
     use_graphs: bool = True
     cache_quant: str | None = None
-    """None (the model dtype) or "fp8": K/V stored as e4m3 with `k_scale` / `v_scale`."""
+    """None (the model dtype), "fp8" (K/V stored as e4m3 with `k_scale` / `v_scale`) or "int8" (8-bit codes with a
+    scale for every block and KV head, which need no scale beforehand)."""
     k_scale: float = 1.0
     v_scale: float = 1.0
 

@@ -15,6 +15,9 @@ RMSNorm and the SiLU-gated MLP (llama.py:101-112) with gate and up stacked.
 On a ROCm device 16-bit projections of up to 256 rows run as this library's
 kernels where those are the faster ones (engine/ops.py), the others as torch
 GEMMs (hipBLASLt); attention, RoPE and the slot-write are this library's kernels.
+With ``weight_quant="int8"`` the layers' projections hold 8-bit weights with a
+scale for each output channel and run as `ops.linear_int8` (the embedding and
+the head stay in the model's dtype).
 """
 
 from __future__ import annotations
@@ -25,6 +28,9 @@ import torch
 import torch.nn.functional as F
 
 from liteinfer_amd.attention import paged_attention
+from liteinfer_amd.engine.ops import Int8Weight, linear_int8, quantize_weight
+
+WEIGHT_QUANT_FORMATS = (None, "int8")
 
 
 @dataclass(frozen=True)
@@ -48,12 +54,13 @@ LLAMA_3_8B = LlamaShape()
 
 
 class _Layer:
-    def __init__(self, shape: LlamaShape, gen: torch.Generator, device, dtype, std: float) -> None:
+    def __init__(self, shape: LlamaShape, gen: torch.Generator, device, dtype, std: float, weight_quant: str | None) -> None:
         h, d = shape.hidden_size, shape.head_dim
         qkv_out = (shape.num_heads + 2 * shape.num_kv_heads) * d
 
         def w(out_f, in_f):
-            return (torch.randn(out_f, in_f, generator=gen, device=device, dtype=torch.float32) * std).to(dtype)
+            weight = (torch.randn(out_f, in_f, generator=gen, device=device, dtype=torch.float32) * std).to(dtype)
+            return quantize_weight(weight) if weight_quant else weight
 
         self.attn_norm = torch.ones(h, device=device, dtype=dtype)
         self.w_qkv = w(qkv_out, h)
@@ -63,18 +70,26 @@ class _Layer:
         self.w_down = w(h, shape.intermediate_size)
 
 
+def _linear(x: torch.Tensor, w: torch.Tensor | Int8Weight) -> torch.Tensor:
+    """A projection in torch ops (8-bit weights: `linear_int8`, which serves either device)."""
+    return linear_int8(x, *w) if isinstance(w, Int8Weight) else F.linear(x, w)
+
+
 class RandomLlama:
     """Seeded random weights of a Llama architecture; `forward` mirrors LlamaForCausalLM.forward."""
 
     def __init__(self, shape: LlamaShape = LLAMA_3_8B, device="cuda", dtype=torch.bfloat16, seed: int = 0,
-                 std: float = 0.02) -> None:
+                 std: float = 0.02, weight_quant: str | None = None) -> None:
+        if weight_quant not in WEIGHT_QUANT_FORMATS:
+            raise ValueError(f"weight_quant must be one of {WEIGHT_QUANT_FORMATS}, got {weight_quant!r}")
+        self.weight_quant = weight_quant
         self.shape = shape
         self.device = torch.device(device)
         self.dtype = dtype
         gen = torch.Generator(device=self.device).manual_seed(seed)
         self.embed = (torch.randn(shape.vocab_size, shape.hidden_size, generator=gen, device=self.device,
                                   dtype=torch.float32) * std).to(dtype)
-        self.layers = [_Layer(shape, gen, self.device, dtype, std) for _ in range(shape.num_layers)]
+        self.layers = [_Layer(shape, gen, self.device, dtype, std, weight_quant) for _ in range(shape.num_layers)]
         self.final_norm = torch.ones(shape.hidden_size, device=self.device, dtype=dtype)
         self.lm_head = (torch.randn(shape.vocab_size, shape.hidden_size, generator=gen, device=self.device,
                                     dtype=torch.float32) * std).to(dtype)
@@ -95,7 +110,9 @@ class RandomLlama:
     def parameter_bytes(self) -> int:
         tensors = [self.embed, self.lm_head, self.final_norm]
         for layer in self.layers:
-            tensors += [layer.attn_norm, layer.w_qkv, layer.w_o, layer.mlp_norm, layer.w_gate_up, layer.w_down]
+            tensors += [layer.attn_norm, layer.mlp_norm]
+            for w in (layer.w_qkv, layer.w_o, layer.w_gate_up, layer.w_down):
+                tensors += w if isinstance(w, Int8Weight) else [w]
         return sum(t.numel() * t.element_size() for t in tensors)
 
     def _rms_norm(self, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -129,7 +146,7 @@ class RandomLlama:
         cos, sin = self._rotary(positions)
         nq, nkv = s.num_heads, s.num_kv_heads
         fused = self._fused_ops
-        linear = fused.linear if fused else F.linear
+        linear = fused.linear if fused else _linear
         delta = None  # the MLP output not yet added to the residual stream
         for idx, layer in enumerate(self.layers):
             if fused:
@@ -147,10 +164,10 @@ class RandomLlama:
                 x = fused.add_rms_norm(h, layer.mlp_norm, s.rms_norm_eps, fused.linear_sums(attn, layer.w_o))
                 delta = fused.linear_sums(fused.gate_up_silu(x, layer.w_gate_up), layer.w_down)
             else:
-                h = h + F.linear(attn, layer.w_o)
+                h = h + _linear(attn, layer.w_o)
                 x = self._rms_norm(h, layer.mlp_norm)
-                gate, up = F.linear(x, layer.w_gate_up).chunk(2, dim=-1)
-                h = h + F.linear(F.silu(gate) * up, layer.w_down)
+                gate, up = _linear(x, layer.w_gate_up).chunk(2, dim=-1)
+                h = h + _linear(F.silu(gate) * up, layer.w_down)
         if fused:
             h = fused.add_rms_norm(h, self.final_norm, s.rms_norm_eps, delta)
         else:

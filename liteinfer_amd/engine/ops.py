@@ -1,6 +1,6 @@
 """The minimal engine's own ops on a ROCm device: fused elementwise work (`li_add_rms_norm`,
-`li_silu_mul`), the decode step's projections (`li_skinny_gemm`) and its inputs (`li_rotary_tables`,
-`li_stage_decode`).
+`li_silu_mul`), the decode step's projections (`li_skinny_gemm`), projections in 8-bit integers (`li_linear_int8`)
+and the step's inputs (`li_rotary_tables`, `li_stage_decode`).
 
 Same results as the model's torch ops (liteinfer/models/llama.py:34-48,
 :101-116) up to the order of the fp32 sum of squares and the exponential's
@@ -47,6 +47,15 @@ class Partials(NamedTuple):
     """The projection's shape, ``[..., n]``."""
 
 
+class Int8Weight(NamedTuple):
+    """A projection's weight in 8 bits: row j of ``[n, k]`` stands for ``codes[j] * scales[j]``."""
+
+    codes: torch.Tensor
+    """int8 ``[n, k]``, rows at multiples of 16 bytes (`quantize_weight` lays them out so)."""
+    scales: torch.Tensor
+    """float32 ``[n]``."""
+
+
 # Rows of x up to which the projections may run as this library's kernels
 # (LI_SKINNY_MAX_ROWS; li_skinny_gemm_plan says which); torch's GEMMs serve
 # the others.
@@ -88,8 +97,10 @@ def _gemm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None, sums: torc
     _native.check(status, "skinny_gemm")
 
 
-def linear_sums(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor | Partials:
+def linear_sums(x: torch.Tensor, w: torch.Tensor | Int8Weight) -> torch.Tensor | Partials:
     """``x @ w.T`` for an op that takes `Partials`: those where the kernel cut K, the rounded rows elsewhere."""
+    if isinstance(w, Int8Weight):
+        return linear_int8(x, *w)
     flat, splits = _skinny(x, w)
     if splits == 0:
         return F.linear(x, w)
@@ -103,7 +114,7 @@ def linear_sums(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor | Partials:
     return out.view(shape)
 
 
-def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+def linear(x: torch.Tensor, w: torch.Tensor | Int8Weight) -> torch.Tensor:
     """``x @ w.T``, the model's projection."""
     got = linear_sums(x, w)
     if not isinstance(got, Partials):
@@ -116,8 +127,10 @@ def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def gate_up_silu(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+def gate_up_silu(x: torch.Tensor, w: torch.Tensor | Int8Weight) -> torch.Tensor:
     """``silu(gate) * up`` of the fused projection ``x @ w.T = [gate | up]``."""
+    if isinstance(w, Int8Weight):
+        return silu_mul(linear_int8(x, *w))
     flat, splits = _skinny(x, w)
     if splits == 0 or w.shape[0] % 16:
         return silu_mul(F.linear(x, w))
@@ -131,6 +144,97 @@ def gate_up_silu(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     status = _native.load().li_silu_mul_partials(sums.data_ptr(), splits, out.data_ptr(), rows, ffn, ffn,
                                                  _native.dtype_code(x.dtype), _native.stream_handle(x.device))
     _native.check(status, "silu_mul")
+    return out
+
+
+def _row_scale(largest: torch.Tensor) -> torch.Tensor:
+    """A row's scale from its largest magnitude: over 127, 2^-126 at least, NaN for what is not finite."""
+    scale = (largest * (1.0 / 127.0)).clamp(min=2.0 ** -126)
+    return torch.where(torch.isfinite(largest), scale, float("nan"))
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x ``[..., k]`` as int8 codes with a float32 scale for each row: ``(codes [..., k], scales [...])``.
+
+    ``scale = max(largest magnitude / 127, 2^-126)``, ``code = rint(x / scale)``
+    in float32; a row with a value that is not finite gets the scale NaN and
+    codes 0. Rows of codes start at multiples of 16 bytes.
+    """
+    if x.dtype not in _native.DTYPE_CODES or x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"quantize_rows takes float32, float16 or bfloat16 rows, got {x.dtype} {list(x.shape)}")
+    k = x.shape[-1]
+    flat = x.reshape(-1, k)
+    if flat.stride(-1) != 1:
+        flat = flat.contiguous()
+    rows, padded = flat.shape[0], -(-k // 16) * 16
+    codes = torch.empty(rows, padded, dtype=torch.int8, device=x.device)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if x.is_cuda:
+        _native.check(_native.on_device(
+            x.device, _native.load().li_quantize_rows, flat.data_ptr(), flat.stride(0) if rows > 1 else k,
+            codes.data_ptr(), padded, scales.data_ptr(), rows, k, padded, _native.dtype_code(x.dtype),
+            _native.stream_handle(x.device)), "quantize_rows")
+    else:
+        wide = flat.to(torch.float32)
+        scales.copy_(_row_scale(wide.abs().amax(dim=-1)))
+        lost = torch.isnan(scales)[:, None]
+        inv = torch.where(lost, 0.0, 1.0 / scales[:, None])
+        codes.zero_()[:, :k] = torch.round(torch.where(lost, 0.0, wide) * inv).clamp(-127, 127).to(torch.int8)
+    return codes[:, :k].view(*x.shape[:-1], k), scales.view(x.shape[:-1])
+
+
+def quantize_weight(w: torch.Tensor) -> Int8Weight:
+    """A projection's weight ``[n, k]`` in 8 bits with a scale for each output channel, as `linear_int8` takes it."""
+    if w.dim() != 2:
+        raise ValueError(f"a weight is [n, k], got {list(w.shape)}")
+    return Int8Weight(*quantize_rows(w))
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_int8_bytes(rows: int, n: int, k: int, device_index: int) -> int:
+    need = ctypes.c_size_t()
+    _native.check(_native.load().li_linear_int8_plan(rows, n, k, ctypes.byref(need)), "linear_int8")
+    return need.value
+
+
+def linear_int8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """``x @ w.T`` in 8-bit integers: x ``[..., k]`` quantised row by row, w ``codes [n, k]`` times ``scales [n]``.
+
+    x's rows are quantised as `quantize_rows` does; products are summed exactly
+    and ``sum * row scale * channel scale`` is rounded once to x's dtype
+    (float32, float16 or bfloat16). A row with a value that is not finite gives
+    NaN. `codes` rows start at multiples of 16 bytes (`quantize_weight`).
+    """
+    if x.dtype not in _native.DTYPE_CODES or x.dim() < 1:
+        raise ValueError(f"linear_int8 takes float32, float16 or bfloat16 rows, got {x.dtype} {list(x.shape)}")
+    if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != x.shape[-1] or 0 in codes.shape:
+        raise ValueError(f"the weight's codes must be int8 [n, {x.shape[-1]}], got {codes.dtype} {list(codes.shape)}")
+    n, k = codes.shape
+    if scales.dtype != torch.float32 or scales.shape != (n,) or (n > 1 and scales.stride(0) != 1):
+        raise ValueError(f"the weight's scales must be contiguous float32 [{n}], got {scales.dtype} {list(scales.shape)}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("linear_int8 has no gradient: call it under torch.no_grad()")
+    if codes.device != x.device or scales.device != x.device:
+        raise ValueError(f"linear_int8 takes tensors on one device, got {[str(t.device) for t in (x, codes, scales)]}")
+    flat = x.reshape(-1, k)
+    if flat.stride(-1) != 1:
+        flat = flat.contiguous()
+    rows = flat.shape[0]
+    if not x.is_cuda:
+        xc, xs = quantize_rows(flat)
+        sums = xc.to(torch.float64) @ codes.to(torch.float64).t()  # whole numbers below 2^31: exact
+        return (sums.to(torch.float32) * xs[:, None] * scales).to(x.dtype).view(*x.shape[:-1], n)
+    stride, padded = codes.stride(0) if n > 1 else -(-k // 16) * 16, -(-k // 16) * 16
+    end = codes.storage_offset() + (n - 1) * stride + padded
+    if (codes.stride(1) != 1 and k > 1) or stride % 16 or stride < padded or codes.data_ptr() % 16 or end > codes.untyped_storage().nbytes():
+        raise ValueError("rows of codes must start at multiples of 16 bytes and be padded to them: quantize_weight lays them out")
+    out = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
+    need = _native.on_device(x.device, _linear_int8_bytes, rows, n, k, x.device.index or 0)
+    workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _native.check(_native.on_device(
+        x.device, _native.load().li_linear_int8, flat.data_ptr(), flat.stride(0) if rows > 1 else k, codes.data_ptr(),
+        stride, scales.data_ptr(), out.data_ptr(), n, rows, n, k, workspace.data_ptr(), need,
+        _native.dtype_code(x.dtype), _native.stream_handle(x.device)), "linear_int8")
     return out
 
 

@@ -68,3 +68,23 @@ def rotate(x: np.ndarray, cos: np.ndarray, sin: np.ndarray, dtype=np.float32) ->
     lo, hi = x[..., :half], x[..., half:]
     return np.concatenate((lo * cos[..., :half] - hi * sin[..., :half],
                            hi * cos[..., half:] + lo * sin[..., half:]), axis=-1)
+
+
+def quantize_rows(x: np.ndarray, dtype=np.float32):
+    """(codes int8 [..., k], scales [...]) of rows: scale = max(largest / 127, 2^-126), code = rint(x * (1 / scale))."""
+    x = x.astype(dtype)
+    largest = np.abs(x).max(axis=-1)
+    step = largest * dtype(1.0 / 127.0) if dtype is np.float32 else largest / 127
+    scales = np.maximum(step, dtype(LEAST))
+    lost = ~np.isfinite(largest)
+    codes = np.clip(np.rint(np.where(lost[..., None], 0, x) * (dtype(1) / scales)[..., None]), -127, 127)
+    codes[lost] = 0
+    return codes.astype(np.int8), np.where(lost, dtype(np.nan), scales).astype(dtype)
+
+
+def linear(x: np.ndarray, codes: np.ndarray, scales: np.ndarray, dtype=np.float32) -> np.ndarray:
+    """x [m, k] times the weight codes [n, k] * scales [n]: whole-number sums, then two products in `dtype`."""
+    xc, xs = quantize_rows(x, dtype)
+    # (Products and sums of whole numbers below 2^53: exact in float64.)
+    sums = xc.astype(np.float64) @ codes.astype(np.float64).T
+    return sums.astype(dtype) * xs[:, None] * scales.astype(dtype)
