@@ -25,7 +25,6 @@ constexpr int kCombineWaves = LI_COMBINE_WAVES;
 template <typename T, int D, int KV>
 __global__ __launch_bounds__(64) void decode_partitioned(AttnArgs a) {
   __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds;
-  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   // Partition-major order: every sequence's first partition is dispatched
   // before any second one, so the grid's empty tail comes last.
   int bid = blockIdx.x;
@@ -56,6 +55,7 @@ __global__ __launch_bounds__(64) void decode_partitioned(AttnArgs a) {
   DecodeState st;
   reset_state(st);
   fold_keys<T, D, KV>(a, lds, q, seq, kvh, kb, ke, st);
+  const float vscale = out_scale<KV>(a, st);
   const int head0 = kvh * a.groups;
   if (nparts == 1) {
     store_state<T, D>(st, static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)head0 * a.o_s1, a.o_s1,
@@ -97,7 +97,6 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
   constexpr int kChunk = kChunkOf<KV>;
   static_assert(HG % 2 == 0, "an even head count keeps every ring stage index a constant");
   __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds_of[P];
-  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   const int lane = threadIdx.x & 63;
   // Wave pw of the work-group folds head group P * grp + pw: the P waves
   // of a work-group walk the same keys of adjacent groups.
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
         }
         if constexpr (KV == kPoolI8) {
           static_assert(HG <= kScaleHeads, "the LDS holds the scales of a group's heads");
-          stage_scales(a, lds, h0, HG);
+          stage_scales<HG>(a, lds, h0, st);
         }
         // The ring runs over (tile, head) pairs; pair ti * HG + h folds from
         // stage h % 2 while the next pair's loads land in the other stage.
@@ -293,6 +292,7 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
       const int slot = first_segment ? 0 : 1;
 #pragma unroll
       for (int h = 0; h < HG; ++h) {
+        const float vscale = out_scale<KV>(a, st[h]);
         if (whole) {
           store_state<T, D>(st[h], static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)(h0 + h) * G * a.o_s1,
                             a.o_s1, nullptr, nullptr, 0, G, vscale);
@@ -593,19 +593,19 @@ __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
   // Each wave's state into its own stages (its loads have drained): head n's
   // accumulator row, its running maximum and its denominator.
   const float lt = li_group_sum(st.l);
+  const float vscale = out_scale<KV>(a, st);
   float* acc = reinterpret_cast<float*>(lds_of[wv].stage);
   if (n < G) {
 #pragma unroll
     for (int blk = 0; blk < D / 16; ++blk)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[n * D + 16 * blk + 4 * g + r] = st.acc[blk][r];
+      for (int r = 0; r < 4; ++r) acc[n * D + 16 * blk + 4 * g + r] = KV == kPoolI8 ? st.acc[blk][r] * vscale : st.acc[blk][r];
     if (g == 0) {
       s_m[wv][n] = st.m;
       s_l[wv][n] = lt;
     }
   }
   __syncthreads();
-  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   T* orow = static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)kvh * G * a.o_s1;
   for (int e = threadIdx.x; e < G * D; e += 64 * NW) {
     const int h = e / D, d = e % D;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(64 * NW) void decode_short(AttnArgs a) {
         num = fmaf(wgt, reinterpret_cast<const float*>(lds_of[v].stage)[h * D + d], num);
         den = fmaf(wgt, s_l[v][h], den);
       }
-      orow[(int64_t)h * a.o_s1 + d] = li_from_float<T>(num * (vscale / den));
+      orow[(int64_t)h * a.o_s1 + d] = li_from_float<T>(num * ((KV == kPoolI8 ? 1.f : vscale) / den));
     }
   }
 }

@@ -124,9 +124,12 @@ struct DecodeLds<D, kPoolI8, kChunk> {
 // Online-softmax state of one wave: lane (n, g) holds head n's running max
 // and (partial) denominator, and in acc[blk][r] (blk < D / 16) dim
 // 16 blk + 4 g + r of its accumulator.
+// int8 pools: the accumulator is in units of vref, a power of two at least
+// the largest of V's scales met so far.
 struct DecodeState {
   float m, l;
   floatx4_t acc[8];
+  float vref;
 };
 
 // The query operand of one KV head's group, as the score MFMAs take it
@@ -298,13 +301,14 @@ struct TileOffsets {
 // into `st`; keys at or past `te` are masked. q holds the group's query, sc
 // the softmax scale times log2(e) (and an fp8 pool's k_scale, and the
 // query's scale q.scale). ks / vs: an int8 pool's scales of the tile's keys,
-// in LDS; the weights of such a pool are rounded to bf16 whatever the query's
-// type, once times their keys' scales: fp16 could not hold those products.
+// in LDS, V's over st.vref (stage_scales): the weights times those are rounded
+// to fp16 whatever the query's type (11 bits, where bf16 has 8; they are at
+// most 2^(kLazyRescale + 1)).
 template <typename T, int D, int KV>
 __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const DecodeQuery<T, D, KV>& q, float sc,
                                           const TileOffsets<D, KV>& o, DecodeState& st, const float* ks = nullptr,
                                           const float* vs = nullptr) {
-  using W = std::conditional_t<KV == kPoolI8, li_bf16, T>;  // the weights' type
+  using W = std::conditional_t<KV == kPoolI8, li_f16, T>;  // the weights' type
   using M = Mfma<W>;
   using Frag = typename M::Frag;
   using L = KvTile<D, KV>;
@@ -408,19 +412,46 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
   }
 }
 
-// An int8 pool's scales of the first `count` staged keys (a multiple of 64)
-// for KV head `kvh` of heads kvh .. kvh + heads - 1, into LDS beside the slots.
-template <int D, int kChunk>
-__device__ __forceinline__ void stage_scales(const AttnArgs& a, DecodeLds<D, kPoolI8, kChunk>& lds, int kvh, int heads) {
+// An int8 pool's scales of the staged keys for KV heads kvh .. kvh + HG - 1,
+// into LDS beside the slots: K's as they are, V's over the head's st.vref,
+// which grows to a power of two at least as large as every scale of the chunk
+// (the accumulator then moves to the new unit: rarely, after the first chunk).
+template <int HG, int D, int kChunk>
+__device__ __forceinline__ void stage_scales(const AttnArgs& a, DecodeLds<D, kPoolI8, kChunk>& lds, int kvh,
+                                             DecodeState* st) {
+  constexpr int kPer = kChunk / 64 + 1;
   const int lane = li_lane();
   const uint32_t bs = (uint32_t)a.block_size;
-#pragma unroll 4
-  for (int k = 0; k < kChunk / 64 + 1; ++k) {
+  float v[HG][kPer], top[HG];
+#pragma unroll
+  for (int h = 0; h < HG; ++h) top[h] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
     const int64_t at = (int64_t)((uint32_t)lds.sl[lane + 64 * k] / bs) * a.sc_s + kvh;
-    for (int h = 0; h < heads; ++h) {
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
       lds.ks[h][lane + 64 * k] = a.ks[at + h];
-      lds.vs[h][lane + 64 * k] = a.vs[at + h];
+      v[h][k] = a.vs[at + h];
+      top[h] = fmaxf(top[h], v[h][k]);
     }
+  }
+#pragma unroll
+  for (int h = 0; h < HG; ++h) {
+    const float t = li_wave_max(top[h]);
+    // The power of two above t (a block that holds NaN is no larger or smaller; t below 2^-126 counts as that).
+    const uint32_t e = min(max(__float_as_uint(t) >> 23, 1u), 253u) + 1;
+    const float unit = __uint_as_float(e << 23);
+    if (unit > st[h].vref) {
+      const float f = st[h].vref / unit;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[h].acc[i][r] *= f;
+      st[h].vref = unit;
+    }
+    const float inv = 1.f / st[h].vref;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) lds.vs[h][lane + 64 * k] = v[h][k] * inv;
   }
 }
 
@@ -454,7 +485,7 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, KV, kC
 #pragma unroll
       for (int k = 0; k < kChunk / 64 + 1; ++k) lds.sl[lane + 64 * k] = vals[k];
     }
-    if constexpr (KV == kPoolI8) stage_scales(a, lds, kvh, 1);
+    if constexpr (KV == kPoolI8) stage_scales<1>(a, lds, kvh, &st);
 
     auto fold = [&](uint32_t stage, int t0) __attribute__((always_inline)) {
       if constexpr (KV == kPoolI8) fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st, lds.ks[0] + (t0 - c0), lds.vs[0] + (t0 - c0));
@@ -551,9 +582,17 @@ __device__ __forceinline__ void store_state(const DecodeState& st, T* orow_head0
   }
 }
 
+// What the accumulator's units stand for: an fp8 pool's V scale, an int8
+// pool's vref.
+template <int KV>
+__device__ __forceinline__ float out_scale(const AttnArgs& a, const DecodeState& st) {
+  return KV == kPoolF8 ? a.v_scale : KV == kPoolI8 ? st.vref : 1.f;
+}
+
 __device__ __forceinline__ void reset_state(DecodeState& st) {
   st.m = -INFINITY;
   st.l = 0.f;
+  st.vref = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) st.acc[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 }
@@ -613,7 +652,6 @@ __device__ __forceinline__ void balanced_share(const AttnArgs& a, int64_t waves,
 // One wave's share of the balanced split: wave w of `waves` (its LDS `lds`).
 template <typename T, int D, int KV>
 __device__ __forceinline__ void decode_balanced_wave(const AttnArgs& a, int w, int64_t waves, DecodeLds<D, KV>& lds) {
-  const float vscale = KV == kPoolF8 ? a.v_scale : 1.f;
   const int lane = li_lane();
   int64_t total, share;
   balanced_share(a, waves, total, share);
@@ -675,6 +713,7 @@ __device__ __forceinline__ void decode_balanced_wave(const AttnArgs& a, int w, i
     DecodeState st;
     reset_state(st);
     fold_keys<T, D, KV>(a, lds, q, seq, kvh, key0, key0 + take, st);
+    const float vscale = out_scale<KV>(a, st);
     if (key0 == 0 && take == ctx) {
       store_state<T, D>(st, static_cast<T*>(a.out) + (int64_t)row * a.o_s0 + (int64_t)kvh * G * a.o_s1, a.o_s1,
                         nullptr, nullptr, 0, G, vscale);

@@ -154,24 +154,28 @@ struct I8Tile64 {
   __device__ static int voffset(int key, int chunk) { return row_of(key) * kRowBytes + 16 * (chunk ^ vswizzle(key)); }
 };
 
-// Eight codes (bytes 0..7 of lo, hi) as a bf16 MFMA operand. A code fits
-// bf16's eight significant bits, so cutting its fp32 form short is exact.
-__device__ __forceinline__ bf16x8_t i8x8_to_bf16(uint32_t lo, uint32_t hi) {
+// Eight codes (bytes 0..7 of lo, hi) as an fp16 MFMA operand, exact: with the
+// sign bit turned, byte u = code + 128 under 0x64 is the fp16 number 1024 + u;
+// less 1152 that is the code (two permutes, two packed adds and half an xor
+// for four codes; through fp32 conversions it would be six).
+__device__ __forceinline__ f16x8_t i8x8_to_f16(uint32_t lo, uint32_t hi) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
   u32x4_t w;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const uint32_t x = (u < 2 ? lo : hi) >> (16 * (u & 1));
-    const uint32_t a = __float_as_uint((float)(int)(int8_t)x), b = __float_as_uint((float)(int)(int8_t)(x >> 8));
-    w[u] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    const uint32_t x = (u < 2 ? lo : hi) ^ 0x80808080u;
+    const uint32_t y = __builtin_amdgcn_perm(0x64646464u, x, (u & 1) ? 0x04030402u : 0x04010400u);
+    w[u] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, y) - bias);
   }
-  return __builtin_bit_cast(bf16x8_t, w);
+  return __builtin_bit_cast(f16x8_t, w);
 }
 
 // The V^T operand of an int8 tile: one 8-bit transposing read at `addr`.
-__device__ __forceinline__ bf16x8_t lds_read_i8_vt(uint32_t addr) {
+__device__ __forceinline__ f16x8_t lds_read_i8_vt(uint32_t addr) {
   typedef int v2i __attribute__((ext_vector_type(2)));
   const v2i v = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)addr);
-  return i8x8_to_bf16((uint32_t)v[0], (uint32_t)v[1]);
+  return i8x8_to_f16((uint32_t)v[0], (uint32_t)v[1]);
 }
 
 // One direct-to-LDS load: every lane's 16 bytes at `g` land at lds + 16 * lane.

@@ -4,11 +4,15 @@ Bounds, per output element, with A = the same attention over |V| (the sum of
 weight times magnitude an element is made of) and h(t) half a step of t
 relative to a value (bf16 2^-8, fp16 2^-11, fp32 2^-24):
 
-* decode, MFMA kernels: the weights times their blocks' scales are rounded to
-  bf16, h(bf16) A; the sum of the weights is not. Scores: the query in 22 bits
-  of its largest value and fp32 products and exponentials, under 2^-14 A for
-  the scores here (|score| < 32: 2^-24 times 32 and log2 e, a few operations
-  over, and D 2^-22 of the largest q k, below 2^-15).
+* decode, MFMA kernels: the weights times their blocks' scales, over the
+  largest scale M met, are rounded to fp16, h(fp16) A, and where they are
+  below its normal range by at most 2^-25: of n keys, whose codes are at most
+  127 and whose weights sum to at least 1, n 2^-25 127 M in all, with M up to
+  twice the largest scale n 2^-24 of the largest |V|. The sum of the weights
+  is not rounded. Scores: the query in 22 bits of its largest value and fp32
+  products and exponentials, under 2^-14 A for the scores here (|score| < 32:
+  2^-24 times 32 and log2 e, a few operations over, and D 2^-22 of the largest
+  q k, below 2^-15).
 * decode and packed passes, general kernel: fp32 throughout, 2^-14 A.
 * packed passes, MFMA kernels: over K and V rounded to the query's dtype (as
   the dense kernels gather them; the oracle is given those), weights rounded
@@ -108,7 +112,8 @@ class Batch:
         assert out.dtype == self.dtype and got.shape == want.shape
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
         moved = self.query_step() if rounded else 0.0
-        bound = (weight_step + moved + 2.0 ** -14) * size + (half_step(self.dtype) + moved + extra) * np.abs(want) * (1 + 2.0 ** -7)
+        small = max(self.contexts) * 2.0 ** -24 * np.nanmax(np.abs(I8.dequantize(self.codes[1], self.scales[1])))
+        bound = small + (weight_step + moved + 2.0 ** -14) * size + (half_step(self.dtype) + moved + extra) * np.abs(want) * (1 + 2.0 ** -7)
         bad = np.abs(got - want) > bound + 1e-30
         assert not bad.any(), (np.abs(got - want)[bad].max(), (np.abs(got - want) / bound)[bad].max(), np.argwhere(bad)[:4])
 
@@ -137,7 +142,7 @@ DECODES = {
 def test_decode(name, kernel, dtype):
     batch = Batch(**DECODES[name], dtype=dtype)
     kw = dict(num_splits=3) if kernel == "equal_splits" else {}
-    batch.check(batch.decode(kernel=kernel, **kw), 0.0 if kernel == "generic" else half_step(BF16))
+    batch.check(batch.decode(kernel=kernel, **kw), 0.0 if kernel == "generic" else half_step(F16))
 
 
 @pytest.mark.parametrize("shape", [dict(dim=80), dict(dim=256), dict(heads=34, kv_heads=2), dict(dtype=F32), dict(dim=33),
@@ -179,9 +184,10 @@ def _check_packed(batch, out):
     copied, copied_size = batch.want(rounded=True)
     got = out.double().cpu().numpy()
     moved = batch.query_step()
-    for want, a, weight, extra, which in ((exact, size, half_step(BF16), 0.0, rows),
+    for want, a, weight, extra, which in ((exact, size, half_step(F16), 0.0, rows),
                                           (copied, copied_size, step + moved, step + moved, ~rows)):
-        bound = (weight + 2.0 ** -14) * a + (step + extra) * np.abs(want) * (1 + 2.0 ** -7)
+        small = max(batch.contexts) * 2.0 ** -24 * np.abs(I8.dequantize(batch.codes[1], batch.scales[1])).max()
+        bound = small + (weight + 2.0 ** -14) * a + (step + extra) * np.abs(want) * (1 + 2.0 ** -7)
         bad = (np.abs(got - want) > bound)[which]
         assert not bad.any(), (np.abs(got - want)[which][bad].max(), np.argwhere(bad)[:4])
     assert np.isfinite(got).all()
@@ -278,10 +284,10 @@ def test_queries_of_very_different_sizes():
         batch.query[:, :, 7] *= 20
         if scale > 1:
             batch.query *= 0.02
-        batch.check(batch.decode(), half_step(BF16))
+        batch.check(batch.decode(), half_step(F16))
     batch = Batch(contexts=[70, 900, 40], width=4000)
     batch.query.zero_()
-    batch.check(batch.decode(), half_step(BF16))
+    batch.check(batch.decode(), half_step(F16))
 
 
 def test_scales_of_very_different_sizes():
@@ -290,7 +296,7 @@ def test_scales_of_very_different_sizes():
         g = np.random.default_rng(5)
         batch.scales[1] *= np.exp(8 * g.normal(size=batch.scales[1].shape)).astype(np.float32)
         batch.scales[0][::3] = 2.0 ** -126
-        batch.check(batch.decode(), half_step(BF16))
+        batch.check(batch.decode(), half_step(F16))
 
 
 def test_slots_past_32_bits_of_bytes():
@@ -306,13 +312,13 @@ def test_slots_past_32_bits_of_bytes():
     for width in (0, 5000):
         table = torch.nn.functional.pad(batch.table_t + far, (0, max(0, width - batch.table.shape[1])))
         out = paged_decode(batch.query, keys, values, table, batch.contexts_t, batch.scaling, 1, key_scales=ks, value_scales=vs)
-        batch.check(out, half_step(BF16))
+        batch.check(out, half_step(F16))
     batch.queries = [1, 1]
     for one_query_rows in (False, True):
         out = paged_prefill(batch.query, keys, values, batch.table_t + far, batch.contexts_t,
                             torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), 1, batch.scaling, 1,
                             one_query_rows=one_query_rows, key_scales=ks, value_scales=vs)
-        batch.check(out, half_step(BF16))
+        batch.check(out, half_step(F16))
     batch = Batch(contexts=[300, 70], queries=[30, 2], heads=8, kv_heads=8, block=64, blocks=5)
     keys[far:], values[far:] = (torch.from_numpy(c).to(DEV) for c in batch.codes)
     ks[-5:], vs[-5:] = (torch.from_numpy(s).to(DEV) for s in batch.scales)
@@ -333,7 +339,7 @@ def test_strided_operands():
     out = paged_decode(query[..., :128], wide[0, :, 1:, 16:144], wide[1, :, 1:, 16:144],
                        batch.table_t.to(torch.int32), batch.contexts_t.long(), batch.scaling, 4,
                        key_scales=scales[0, :, 2:4], value_scales=scales[1, :, 2:4])
-    batch.check(out, half_step(BF16))
+    batch.check(out, half_step(F16))
 
 
 def test_a_sequence_of_operators_as_a_layer_runs_them():
@@ -396,7 +402,7 @@ def test_a_captured_step_replays_for_other_contexts():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, call())
-            batch.check(out, half_step(BF16))
+            batch.check(out, half_step(F16))
 
 
 def test_two_calls_on_two_streams():
@@ -411,7 +417,7 @@ def test_two_calls_on_two_streams():
             outs.append(paged_decode(b.query, k, v, t, c, b.scaling, b.groups, key_scales=ks, value_scales=vs))
     torch.cuda.synchronize()
     for b, out in zip(batches, outs):
-        b.check(out, half_step(BF16))
+        b.check(out, half_step(F16))
 
 
 def test_refusals():
