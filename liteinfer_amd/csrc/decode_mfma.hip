@@ -92,16 +92,17 @@ __global__ __launch_bounds__(64) void decode_balanced(AttnArgs a) {
 // keys.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int KV, int HG, int P>
-__global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
+__global__ __launch_bounds__(64 * P, KV == kPoolI8 ? 2 : 1) void decode_grouped(AttnArgs a) {
   using L = KvTile<D, KV>;
   constexpr int kChunk = kChunkOf<KV>;
-  static_assert(HG % 2 == 0, "an even head count keeps every ring stage index a constant");
-  __shared__ __attribute__((aligned(1024))) DecodeLds<D, KV> lds_of[P];
+  static_assert(HG % 2 == 0 || KV == kPoolI8, "an even head count keeps every ring stage index a constant");
+  using Lds = std::conditional_t<KV == kPoolI8, GroupedI8Lds<D>, DecodeLds<D, KV>>;
+  __shared__ __attribute__((aligned(1024))) Lds lds_of[P];
   const int lane = threadIdx.x & 63;
   // Wave pw of the work-group folds head group P * grp + pw: the P waves
   // of a work-group walk the same keys of adjacent groups.
   const int pw = P > 1 ? (int)(threadIdx.x >> 6) : 0;
-  DecodeLds<D, KV>& lds = lds_of[pw];
+  Lds& lds = lds_of[pw];
   const int w = blockIdx.x;
   const int ngroups = a.num_kv_heads / (HG * P);
   // Work is counted in units: a segment (sequence, group of HG KV heads)
@@ -224,6 +225,10 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
           }
         }
       }
+      if constexpr (KV == kPoolI8) {
+        static_assert(HG == 1, "a wave folds one head of an int8 pool");
+        fold_keys_i8<T, D>(a, lds_addr(lds_of) + pw * (uint32_t)sizeof(Lds), q[0], srow, h0, kb, ke, sc, off, st[0]);
+      } else
       for (int c0 = kb; c0 < ke; c0 += kChunk) {
         const int c1 = min(c0 + kChunk, ke);
         const int ntiles = (c1 - c0 + 31) / 32;
@@ -233,10 +238,6 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
           for (int k = 0; k < kChunk / 64 + 1; ++k) vals[k] = (int)srow[min(c0 + lane + 64 * k, c1 - 1)];
 #pragma unroll
           for (int k = 0; k < kChunk / 64 + 1; ++k) lds.sl[lane + 64 * k] = vals[k];
-        }
-        if constexpr (KV == kPoolI8) {
-          static_assert(HG <= kScaleHeads, "the LDS holds the scales of a group's heads");
-          stage_scales<HG>(a, lds, h0, st);
         }
         // The ring runs over (tile, head) pairs; pair ti * HG + h folds from
         // stage h % 2 while the next pair's loads land in the other stage.
@@ -268,11 +269,7 @@ __global__ __launch_bounds__(64 * P) void decode_grouped(AttnArgs a) {
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
               }
             }
-            if constexpr (KV == kPoolI8)
-              fold_tile<T, D, KV>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h],
-                                  lds.ks[h] + 32 * ti, lds.vs[h] + 32 * ti);
-            else
-              fold_tile<T, D, KV>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h]);
+            fold_tile<T, D, KV>(lds_addr(lds.stage[h & 1]), c0 + 32 * ti, c1, q[h], sc * q[h].scale, off, st[h]);
           }
         }
         li_wait_vm<0>();
@@ -652,14 +649,18 @@ int launch_decode_mfma(const AttnArgs& a, int dtype, hipStream_t s) {
   if (blocks == 0) return LI_OK;
   if (blocks > 0x7fffffffLL) return fail(LI_EUNSUPPORTED, "decode grid of %lld blocks is too large", (long long)blocks);
   const dim3 grid((unsigned)blocks), block(64);
+  // Waves of a work-group and KV heads of a wave: kDecodeHeadGroup heads a
+  // wave, an int8 pool's one a wave and as many more waves.
+#define LI_GROUPED(T, D, KV, P)                                                                               \
+  do {                                                                                                        \
+    constexpr int kHg = KV == kPoolI8 ? 1 : kDecodeHeadGroup, kP = P * kDecodeHeadGroup / kHg;                \
+    hipLaunchKernelGGL((decode_grouped<T, D, KV, kHg, kP>), grid, dim3(64 * kP), 0, s, a);                    \
+  } while (0)
 #define LI_DECODE_LAUNCH(T, D, KV)                                                                   \
   do {                                                                                               \
-    if (balanced && a.part_heads == kDecodeHeadGroup)                                                \
-      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 1>), grid, block, 0, s, a);     \
-    else if (balanced && a.part_heads == 2 * kDecodeHeadGroup)                                       \
-      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 2>), grid, dim3(128), 0, s, a); \
-    else if (balanced && a.part_heads == 4 * kDecodeHeadGroup)                                       \
-      hipLaunchKernelGGL((decode_grouped<T, D, KV, kDecodeHeadGroup, 4>), grid, dim3(256), 0, s, a); \
+    if (balanced && a.part_heads == kDecodeHeadGroup) LI_GROUPED(T, D, KV, 1);                       \
+    else if (balanced && a.part_heads == 2 * kDecodeHeadGroup) LI_GROUPED(T, D, KV, 2);              \
+    else if (balanced && a.part_heads == 4 * kDecodeHeadGroup) LI_GROUPED(T, D, KV, 4);              \
     else if (balanced) hipLaunchKernelGGL((decode_balanced<T, D, KV>), grid, block, 0, s, a);        \
     else hipLaunchKernelGGL((decode_partitioned<T, D, KV>), grid, block, 0, s, a);                   \
   } while (0)
@@ -682,6 +683,7 @@ int launch_decode_mfma(const AttnArgs& a, int dtype, hipStream_t s) {
     else LI_DECODE_LAUNCH(li_f16, 64, kPool16);
   }
 #undef LI_DECODE_LAUNCH
+#undef LI_GROUPED
   if (int rc = check_launch("decode_mfma")) return rc;
   return balanced ? launch_combine_balanced(a, dtype, s) : LI_OK;
 }

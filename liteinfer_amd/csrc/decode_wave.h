@@ -70,32 +70,40 @@ constexpr int kPoolBytes = KV == kPool16 ? (int)sizeof(T) : 1;
 // (rr, n) = (lane / CH, lane % CH) loads keys rr * kInsts + i. kpool / vpool
 // point at the KV head's row of slot 0, row_bytes is the pool's slot stride.
 template <int D, int KV>
-__device__ __forceinline__ void issue_tile(char* stage, const char* __restrict__ kpool,
-                                           const char* __restrict__ vpool, const int* __restrict__ sl,
-                                           uint32_t row_bytes, int t, int lane) {
+__device__ __forceinline__ void issue_tile_at(uint32_t stage, const char* __restrict__ kpool,
+                                              const char* __restrict__ vpool, uint32_t sl, uint32_t row_bytes,
+                                              int lane) {
   using L = KvTile<D, KV>;
   const int rr = lane / L::kCh, nn = lane % L::kCh;
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  typedef int i2 __attribute__((ext_vector_type(2)));
   int keys[L::kInsts];
   if constexpr (L::kInsts == 8) {
-    const int4 a = *reinterpret_cast<const int4*>(sl + t + 8 * rr);
-    const int4 b = *reinterpret_cast<const int4*>(sl + t + 8 * rr + 4);
+    const i4 a = lds_read_frag<i4>(sl + 32 * rr);
+    const i4 b = lds_read_frag<i4>(sl + 32 * rr + 16);
     keys[0] = a.x; keys[1] = a.y; keys[2] = a.z; keys[3] = a.w;
     keys[4] = b.x; keys[5] = b.y; keys[6] = b.z; keys[7] = b.w;
   } else if constexpr (L::kInsts == 4) {
-    const int4 a = *reinterpret_cast<const int4*>(sl + t + 4 * rr);
+    const i4 a = lds_read_frag<i4>(sl + 16 * rr);
     keys[0] = a.x; keys[1] = a.y; keys[2] = a.z; keys[3] = a.w;
   } else {
-    const int2 a = *reinterpret_cast<const int2*>(sl + t + 2 * rr);
+    const i2 a = lds_read_frag<i2>(sl + 8 * rr);
     keys[0] = a.x; keys[1] = a.y;
   }
 #pragma unroll
   for (int i = 0; i < L::kInsts; ++i) {
     const int key = rr * L::kInsts + i;
-    const uint32_t dst = lds_addr(stage + i * 1024);  // rows kRowsPerInst * i ..: 1 KiB per instruction
+    const uint32_t dst = stage + i * 1024;  // rows kRowsPerInst * i ..: 1 KiB per instruction
     // Lane nn writes slot nn of its row: global chunk nn ^ swizzle(key).
     dma16<kDecodeStream>(row_ptr(kpool + 16 * (nn ^ L::kswizzle(key)), (uint32_t)keys[i], row_bytes), dst);
     dma16<kDecodeStream>(row_ptr(vpool + 16 * (nn ^ L::vswizzle(key)), (uint32_t)keys[i], row_bytes), dst + 32 * L::kRowBytes);
   }
+}
+template <int D, int KV>
+__device__ __forceinline__ void issue_tile(char* stage, const char* __restrict__ kpool,
+                                           const char* __restrict__ vpool, const int* __restrict__ sl,
+                                           uint32_t row_bytes, int t, int lane) {
+  issue_tile_at<D, KV>(lds_addr(stage), kpool, vpool, lds_addr(sl + t), row_bytes, lane);
 }
 
 // Keys a wave of the balanced and partitioned kernels stages at a time. An
@@ -112,7 +120,7 @@ struct DecodeLds {
 };
 // int8 pools: the staged keys' scales too, for each of the kScaleHeads KV
 // heads that the wave folds side by side.
-constexpr int kScaleHeads = kDecodeHeadGroup;
+constexpr int kScaleHeads = 1;
 template <int D, int kChunk>
 struct DecodeLds<D, kPoolI8, kChunk> {
   int sl[kChunk + 64];
@@ -300,14 +308,13 @@ struct TileOffsets {
 // Folds the 32-key tile in `stage` (LDS byte address) whose first key is t0
 // into `st`; keys at or past `te` are masked. q holds the group's query, sc
 // the softmax scale times log2(e) (and an fp8 pool's k_scale, and the
-// query's scale q.scale). ks / vs: an int8 pool's scales of the tile's keys,
-// in LDS, V's over st.vref (stage_scales): the weights times those are rounded
+// query's scale q.scale). ks / vs: an int8 pool's scales of the tile's keys
+// (LDS byte addresses), V's over st.vref (stage_scales): the weights times those are rounded
 // to fp16 whatever the query's type (11 bits, where bf16 has 8; they are at
 // most 2^(kLazyRescale + 1)).
 template <typename T, int D, int KV>
 __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const DecodeQuery<T, D, KV>& q, float sc,
-                                          const TileOffsets<D, KV>& o, DecodeState& st, const float* ks = nullptr,
-                                          const float* vs = nullptr) {
+                                          const TileOffsets<D, KV>& o, DecodeState& st, uint32_t ks = 0, uint32_t vs = 0) {
   using W = std::conditional_t<KV == kPoolI8, li_f16, T>;  // the weights' type
   using M = Mfma<W>;
   using Frag = typename M::Frag;
@@ -331,8 +338,7 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
         p1[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k1, q.t[d][j], p1[d], 0, 0, 0);
       }
     }
-    const floatx4_t ks0 = *reinterpret_cast<const floatx4_t*>(ks + 4 * g);
-    const floatx4_t ks1 = *reinterpret_cast<const floatx4_t*>(ks + 16 + 4 * g);
+    const floatx4_t ks0 = lds_read_frag<floatx4_t>(ks + 16 * g), ks1 = lds_read_frag<floatx4_t>(ks + 64 + 16 * g);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       s0[r] = fmaf((float)(p0[0][r] * 256 + p0[1][r]), 256.f, (float)p0[2][r]) * ks0[r];
@@ -390,8 +396,7 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
   }
   st.m = mnew;
   if constexpr (KV == kPoolI8) {
-    const floatx4_t vs0 = *reinterpret_cast<const floatx4_t*>(vs + 4 * g);
-    const floatx4_t vs1 = *reinterpret_cast<const floatx4_t*>(vs + 16 + 4 * g);
+    const floatx4_t vs0 = lds_read_frag<floatx4_t>(vs + 16 * g), vs1 = lds_read_frag<floatx4_t>(vs + 64 + 16 * g);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       p[r] *= vs0[r];
@@ -410,6 +415,24 @@ __device__ __forceinline__ void fold_tile(uint32_t stage, int t0, int te, const 
     else if constexpr (KV == kPoolF8) st.acc[blk] = M::mma(lds_read_f8_vt<Frag>(vstage + o.voff[blk]), pf, st.acc[blk]);
     else st.acc[blk] = M::mma(lds_read_vt<Frag>(vstage + o.voff[blk], vstage + o.voff[blk] + L::kRow16), pf, st.acc[blk]);
   }
+}
+
+// Grows st.vref to a power of two above every lane's `top` (a NaN counts as
+// nothing, what is below 2^-126 as that) and moves the accumulator to the new
+// unit: rarely, after a context's first keys. Returns 1 / st.vref, exact.
+template <int D>
+__device__ __forceinline__ float grow_unit(DecodeState& st, float top) {
+  const uint32_t e = min(max(__float_as_uint(li_wave_max(top)) >> 23, 1u), 253u) + 1;
+  const float unit = __uint_as_float(e << 23);
+  if (unit > st.vref) {
+    const float f = st.vref / unit;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st.acc[i][r] *= f;
+    st.vref = unit;
+  }
+  return 1.f / st.vref;
 }
 
 // An int8 pool's scales of the staged keys for KV heads kvh .. kvh + HG - 1,
@@ -437,19 +460,7 @@ __device__ __forceinline__ void stage_scales(const AttnArgs& a, DecodeLds<D, kPo
   }
 #pragma unroll
   for (int h = 0; h < HG; ++h) {
-    const float t = li_wave_max(top[h]);
-    // The power of two above t (a block that holds NaN is no larger or smaller; t below 2^-126 counts as that).
-    const uint32_t e = min(max(__float_as_uint(t) >> 23, 1u), 253u) + 1;
-    const float unit = __uint_as_float(e << 23);
-    if (unit > st[h].vref) {
-      const float f = st[h].vref / unit;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[h].acc[i][r] *= f;
-      st[h].vref = unit;
-    }
-    const float inv = 1.f / st[h].vref;
+    const float inv = grow_unit<D>(st[h], top[h]);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) lds.vs[h][lane + 64 * k] = v[h][k] * inv;
   }
@@ -488,7 +499,8 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, KV, kC
     if constexpr (KV == kPoolI8) stage_scales<1>(a, lds, kvh, &st);
 
     auto fold = [&](uint32_t stage, int t0) __attribute__((always_inline)) {
-      if constexpr (KV == kPoolI8) fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st, lds.ks[0] + (t0 - c0), lds.vs[0] + (t0 - c0));
+      if constexpr (KV == kPoolI8) fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st, lds_addr(lds.ks[0]) + 4 * (t0 - c0),
+                                                              lds_addr(lds.vs[0]) + 4 * (t0 - c0));
       else fold_tile<T, D, KV>(stage, t0, c1, q, sc, off, st);
     };
 
@@ -511,6 +523,105 @@ __device__ __forceinline__ void fold_keys(const AttnArgs& a, DecodeLds<D, KV, kC
     // Drain the look-ahead loads before the slots (and stages) are reused.
     li_wait_vm<0>();
   }
+}
+
+// The head-grouped decode's keys of an int8 pool: one wave's KV head, with
+// nothing drained between chunks. A tile of codes is half the bytes of a
+// 16-bit one, takes more instructions (its scores are joined from three
+// digits, V is widened, both are scaled), and needs scales as well as slots.
+// So twice as many waves share a CU, two on a SIMD, one head each instead of
+// two (64 sequences of 512 .. 8192 keys, 32 / 8 heads, head_dim 128: kernel
+// 104 -> KERNEL us), and slots and scales come by direct-to-LDS loads of
+// their own, two chunks and one chunk ahead, counted in with the tiles'
+// (staged a chunk at a time a wave stopped for two round trips every chunk).
+constexpr int kI8Chunk = 128;   // keys whose slots and scales are loaded at a time
+constexpr int kI8Slots = 512;   // slots held: a ring of four chunks
+template <int D>
+struct GroupedI8Lds {
+  // Byte offsets of a wave's part: kRing stages, the slots, the scales of two
+  // chunks (K's, V's).
+  static constexpr int kRing = D == 64 ? 4 : 2;
+  static constexpr int kStageBytes = KvTile<D, kPoolI8>::kTileBytes;
+  static constexpr int kSl = kRing * kStageBytes, kKs = kSl + 4 * kI8Slots, kVs = kKs + 8 * kI8Chunk;
+  char bytes[kVs + 8 * kI8Chunk];
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void fold_keys_i8(const AttnArgs& a, uint32_t lds, const DecodeQuery<T, D, kPoolI8>& q,
+                                             const int64_t* srow, int kvh, int kb, int ke, float sc,
+                                             const TileOffsets<D, kPoolI8>& off, DecodeState& st) {
+  using L = KvTile<D, kPoolI8>;
+  using B = GroupedI8Lds<D>;
+  constexpr int R = B::kRing;
+  constexpr int kPer = 2 * L::kInsts;                // loads of a tile
+  constexpr int kMeta = kI8Chunk / 64 * 3;           // loads of a chunk's slots and scales
+  constexpr int kTiles = kI8Chunk / 32;
+  static_assert(kTiles % R == 0 && (R - 1) * kPer + kMeta < 64, "constant stages; vmcnt range");
+  typedef __attribute__((address_space(3))) float lds_float;
+  const int lane = li_lane();
+  const char* kpool = static_cast<const char*>(a.kp) + kvh * a.p_s1;
+  const char* vpool = static_cast<const char*>(a.vp) + kvh * a.p_s1;
+  const uint32_t row_bytes = (uint32_t)a.p_s0, bs = (uint32_t)a.block_size;
+  const uint32_t sl = lds + B::kSl, ks = lds + B::kKs, vs = lds + B::kVs;
+  auto scales_at = [](int chunk, int key) { return 4u * ((chunk & 1) * kI8Chunk + key); };
+  // Keys past the last repeat it, so that every load reads a real row.
+  auto load_slots = [&](int chunk) {
+#pragma unroll
+    for (int u = 0; u < kI8Chunk / 64; ++u) {
+      const int at = chunk * kI8Chunk + 64 * u;
+      dma4(srow + min(kb + at + lane, ke - 1), sl + 4 * (at & (kI8Slots - 1)));
+    }
+  };
+  auto load_scales = [&](int chunk) {
+#pragma unroll
+    for (int u = 0; u < kI8Chunk / 64; ++u) {
+      const int slot = lds_read_frag<int>(sl + 4 * ((chunk * kI8Chunk + 64 * u + lane) & (kI8Slots - 1)));
+      const int64_t at = (int64_t)((uint32_t)slot / bs) * a.sc_s + kvh;
+      dma4(a.ks + at, ks + scales_at(chunk, 64 * u));
+      dma4(a.vs + at, vs + scales_at(chunk, 64 * u));
+    }
+  };
+  auto load_tile = [&](int stage, int tile) {
+    issue_tile_at<D, kPoolI8>(lds + stage * B::kStageBytes, kpool, vpool, sl + 4 * ((32 * tile) & (kI8Slots - 1)),
+                              row_bytes, lane);
+  };
+  const int tiles = (ke - kb + 31) / 32;
+  load_slots(0);
+  load_slots(1);
+  li_wait_vm<0>();
+  load_scales(0);
+#pragma unroll
+  for (int t = 0; t < R - 1; ++t) load_tile(t, t);
+  for (int chunk = 0; chunk * kTiles < tiles; ++chunk) {
+    li_wait_vm<(R - 1) * kPer>();  // this chunk's scales (only its first tiles are newer)
+    {
+      float v[kI8Chunk / 64], top = 0.f;
+#pragma unroll
+      for (int u = 0; u < kI8Chunk / 64; ++u) {
+        v[u] = lds_read_frag<float>(vs + scales_at(chunk, 64 * u + lane));
+        top = fmaxf(top, v[u]);
+      }
+      const float inv = grow_unit<D>(st, top);
+#pragma unroll
+      for (int u = 0; u < kI8Chunk / 64; ++u)
+        *(lds_float*)(uintptr_t)(vs + scales_at(chunk, 64 * u + lane)) = v[u] * inv;
+    }
+    load_scales(chunk + 1);
+    load_slots(chunk + 2);
+    const int left = min(kTiles, tiles - chunk * kTiles);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      if (t >= left) break;
+      load_tile((t + R - 1) % R, chunk * kTiles + t + R - 1);
+      // Newer than this tile: the next R - 1, and, for the tiles loaded
+      // before them, the slots and scales above.
+      if (t < R - 1) li_wait_vm<(R - 1) * kPer + kMeta>();
+      else li_wait_vm<(R - 1) * kPer>();
+      fold_tile<T, D, kPoolI8>(lds + (t % R) * B::kStageBytes, kb + 32 * (chunk * kTiles + t), ke, q, sc * q.scale, off,
+                               st, ks + scales_at(chunk, 32 * t), vs + scales_at(chunk, 32 * t));
+    }
+  }
+  li_wait_vm<0>();  // the look-ahead's loads, before the LDS is used again
 }
 
 // Loads the query operand of KV head `kvh`'s group for the query at `row`.

@@ -211,6 +211,19 @@ __device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
   }
 }
 
+// The same for one dword a lane: lane l's 4 bytes at its `g` land at lds + 4 l.
+__device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "global_load_lds_dword %2, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(g)
+      : "memory");
+}
+
 // A work-group barrier that orders LDS only: this wave's LDS operations are
 // complete when it arrives, and nothing waits for its global loads or
 // stores (__syncthreads' release fence would wait for every one of them).
