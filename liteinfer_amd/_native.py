@@ -232,7 +232,7 @@ class _PythonCalls:
     def decode(*_args):
         return None
 
-    prefill = rope = decode
+    prefill = rope = decode_int8 = prefill_int8 = rope_int8 = linear_int8 = decode
 
 
 def _load_fast_calls(path: Path):
@@ -271,6 +271,9 @@ def fast_calls():
             module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
                 "li_paged_decode_plan", "li_paged_decode_write", "li_paged_prefill_plan", "li_paged_prefill_ex",
                 "li_rope_kv_write", "li_rope_kv_write_fp8")))
+            module.bind_int8(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+                "li_paged_decode_int8", "li_paged_prefill_int8_plan", "li_paged_prefill_int8", "li_rope_kv_write_int8",
+                "li_linear_int8_plan", "li_linear_int8")))
             _fast = module
     return _fast
 
@@ -289,9 +292,14 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(message)
 
 
+def is_current(device: torch.device) -> bool:
+    """Whether launches go to `device`."""
+    return device.index is None or device.index == torch.cuda.current_device()
+
+
 def on_device(device: torch.device, call, *args) -> int:
     """`call(*args)` with `device` current: a launch goes to the current device, whatever stream it is given."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if is_current(device):
         return call(*args)
     with torch.cuda.device(device):
         return call(*args)

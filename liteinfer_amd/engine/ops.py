@@ -205,6 +205,13 @@ def linear_int8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> t
     (float32, float16 or bfloat16). A row with a value that is not finite gives
     NaN. `codes` rows start at multiples of 16 bytes (`quantize_weight`).
     """
+    if x.is_cuda and _native.is_current(x.device):
+        # Operands that need no conversion: checked and passed on in C++.
+        out = _native.fast_calls().linear_int8(x, codes, scales, _native.stream_handle(x.device))
+        if out is not None:
+            if isinstance(out, int):
+                _native.check(out, "linear_int8")
+            return out
     if x.dtype not in _native.DTYPE_CODES or x.dim() < 1:
         raise ValueError(f"linear_int8 takes float32, float16 or bfloat16 rows, got {x.dtype} {list(x.shape)}")
     if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != x.shape[-1] or 0 in codes.shape:

@@ -424,6 +424,15 @@ def paged_decode(
             if isinstance(out, int):
                 _native.check(out, "paged_decode")
             return out
+    elif (query.is_cuda and key_scales is not None and new_key is None and new_value is None and kernel in _FLAGS
+          and (num_splits is None or num_splits > 0) and _native.is_current(query.device)):
+        out = _native.fast_calls().decode_int8(
+            query, key_pool, value_pool, slot_table, context_lens, key_scales, value_scales, scaling, num_kv_groups,
+            block_kv, num_splits or 0, _FLAGS[kernel], _native.stream_handle(query.device))
+        if out is not None:
+            if isinstance(out, int):
+                _native.check(out, "paged_decode")
+            return out
     device, query, slot_table, context_lens, kv_code = _decode_inputs(
         query, key_pool, value_pool, slot_table, context_lens, num_kv_groups, num_splits, k_scale, v_scale)
     batch, num_heads, head_dim = query.shape
@@ -603,6 +612,17 @@ def paged_prefill(
         got = _native.fast_calls().prefill(
             query, key_pool, value_pool, slot_table, context_lens, query_start_loc, max_query_len, scaling,
             num_kv_groups, block_kv, block_q, flags, k_scale, v_scale, out, _native.stream_handle(query.device))
+        if got is not None:
+            if isinstance(got, int):
+                _native.check(got, "paged_prefill")
+            return got
+    elif query.is_cuda and key_scales is not None and kernel in ("auto", "generic") and _native.is_current(query.device):
+        flags = _FLAGS[kernel] | (_native.LI_FLAG_PREFILL_ONLY if one_query_rows is False else 0)
+        tokens = context_lens.numel() * slot_table.shape[-1] if context_tokens is None else context_tokens
+        got = _native.fast_calls().prefill_int8(
+            query, key_pool, value_pool, slot_table, context_lens, query_start_loc, key_scales, value_scales,
+            max_query_len, tokens, scaling, num_kv_groups, block_kv, block_q, flags, out,
+            _native.stream_handle(query.device))
         if got is not None:
             if isinstance(got, int):
                 _native.check(got, "paged_prefill")

@@ -86,6 +86,13 @@ def rope_kv_write(
             if isinstance(out, int):
                 _native.check(out, "rope_kv_write")
             return out
+    elif q.is_cuda and _native.is_current(q.device):
+        out = _native.fast_calls().rope_int8(q, k, v, cos, sin, slots, key_pool, value_pool, key_scales, value_scales,
+                                             bad_slots, _native.stream_handle(q.device))
+        if out is not None:
+            if isinstance(out, int):
+                _native.check(out, "rope_kv_write")
+            return out
     device = _require_device_tensors(q, k, v, cos, sin, slots, key_pool, value_pool)
     bad_ptr = bad_slots_pointer(bad_slots, device)
     _check_pools(key_pool, value_pool)
