@@ -19,6 +19,8 @@
 // held to its rows' last 16 bytes.
 #include "li_mfma.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace li;
@@ -141,6 +143,7 @@ struct GemmArgs {
   int m, n, k;
   int splits;
   int vec;           // four outputs side by side may be stored at once
+  int rows16;        // 16-bit rows of the output are 16-byte aligned
   int mt, nt;        // tiles of rows of x, of w
 };
 
@@ -187,15 +190,36 @@ __device__ __forceinline__ void wait_stages(int newer) {
   else li_wait_vm<0>();
 }
 
+// This work-group's tile: {tile of x's rows x runs + run, tile of w's rows}.
+// Work-group i runs on XCD i % 8; each XCD takes a run of tiles, side by side
+// along x's rows first, so that its L2 serves a tile of w to several.
+__device__ __forceinline__ int2 tile_of(const GemmArgs& a, int splits) {
+  const int across = a.mt * splits, total = across * a.nt;
+  const int per = total / 8, rest = total % 8;
+  const int xcd = (int)(blockIdx.x % 8u), at = (int)(blockIdx.x / 8u);
+  const int t = xcd * per + min(xcd, rest) + at;
+  return int2{t % across, t / across};
+}
+
 // A work-group of WM x WN waves takes BM rows of x by BN rows of w and a run
 // of k, both operands straight into LDS in a ring of R stages of RB bytes a
-// row: chunk c (16 bytes) of row r at c ^ (r / (256 / RB)) % (RB / 16), so that
-// the 16 rows an operand read spans lie in 16 different bank groups. R - 1
-// stages are in flight, one barrier a stage.
+// row, chunk c (16 bytes) of row r at c ^ swizzle(r). A 16-byte LDS read is
+// served 16 lanes at a time, lanes 0-3, 12-15, 20-23 and 24-27 together, then
+// 4-11, 16-19 and 28-31, then the same of the upper half: eight rows of one
+// chunk with eight others of the next, which the swizzles keep in 16 different
+// bank groups (with rows of 64 bytes swizzled by r / 4 every read took twice
+// its time). R - 1 stages are in flight, one barrier a stage; the operands of
+// one step of 64 k are read while the step before is multiplied, across the
+// barrier too, one read with every few products.
+template <int RB>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (RB == 64) return (0x78 >> (2 * ((row >> 2) & 3))) & 3;  // 0, 2, 3, 1
+  else return (row / (256 / RB)) % (RB / 16);
+}
 template <typename T, int BM, int BN, int WM, int WN, int RB, int R>
 __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
   constexpr int kWaves = WM * WN;
-  constexpr int kCh = RB / 16, kQ = 256 / RB;  // chunks of a row, rows of a 256-byte bank row
+  constexpr int kCh = RB / 16;                 // chunks of a row
   constexpr int kRows = 64 / kCh;              // rows one load fills
   constexpr int kLoads = (BM + BN) / kRows, kPer = kLoads / kWaves;
   static_assert(kPer >= 1 && kPer * kWaves == kLoads, "the waves split a stage's loads evenly");
@@ -206,14 +230,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r16 = lane & 15, g = lane >> 4;
 
-  // Work-group i runs on XCD i % 8; each XCD takes a run of tiles, side by
-  // side along x's rows first, so that its L2 serves a tile of w to several.
-  const int total = a.mt * a.nt * a.splits;
-  const int per = total / 8, rest = total % 8;
-  const int xcd = (int)(blockIdx.x % 8u), at = (int)(blockIdx.x / 8u);
-  const int t = xcd * per + min(xcd, rest) + at;
-  const int split = t % a.splits, tile = t / a.splits;
-  const int tm = tile % a.mt, tn = tile / a.mt;
+  const int2 tile = tile_of(a, a.splits);
+  const int split = (int)(tile.x % (unsigned)a.splits), tm = (int)(tile.x / (unsigned)a.splits), tn = tile.y;
   const int stages = (a.k + RB - 1) / RB;
   const int s0 = (int)((int64_t)stages * split / a.splits), s1 = (int)((int64_t)stages * (split + 1) / a.splits);
   const int ns = s1 - s0;
@@ -225,7 +243,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int row = kRows * (wv * kPer + i) + lane / kCh;
-    col[i] = 16 * ((lane % kCh) ^ ((row / kQ) % kCh)) + s0 * RB;
+    col[i] = 16 * ((lane % kCh) ^ swizzle<RB>(row)) + s0 * RB;
     src[i] = row < BM ? a.x + (int64_t)min(tm * BM + row, a.m - 1) * a.x_s
                       : a.w + (int64_t)min(tn * BN + row - BM, a.n - 1) * a.w_s;
     // w's rows end at their last chunk; x's go on in zeros.
@@ -246,37 +264,250 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
   const int wm = wv % WM, wn = wv / WM;
   uint32_t off[kK];
 #pragma unroll
-  for (int j = 0; j < kK; ++j) off[j] = (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ ((r16 / kQ) % kCh)));
+  for (int j = 0; j < kK; ++j) off[j] = (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ swizzle<RB>(r16)));
+
+  v4i x0[kFm], w0[kFn], x1[kFm] = {}, w1[kFn] = {};
+  auto read = [&](int st, int j, v4i (&xf)[kFm], v4i (&wf)[kFn]) __attribute__((always_inline)) {
+    const uint32_t stage = base + (uint32_t)(st % R) * kStage + off[j];
+    const uint32_t xc = stage + (uint32_t)wm * (BM / WM) * RB, wc = stage + (uint32_t)(BM + wn * (BN / WN)) * RB;
+#pragma unroll
+    for (int f = 0; f < kFn; ++f) wf[f] = lds_read_frag<v4i>(wc + f * 16 * RB);
+#pragma unroll
+    for (int i = 0; i < kFm; ++i) xf[i] = lds_read_frag<v4i>(xc + i * 16 * RB);
+  };
+  auto multiply = [&](const v4i (&xf)[kFm], const v4i (&wf)[kFn]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kFm; ++i)
+#pragma unroll
+      for (int f = 0; f < kFn; ++f) acc[i][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f], xf[i], acc[i][f], 0, 0, 0);
+  };
+  auto interleave = [&]() __attribute__((always_inline)) {
+    constexpr int kReads = kFm + kFn, kEach = (kFm * kFn + kReads - 1) / kReads;
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    }
+  };
+  // Stage st has landed; every wave is done with stage st - 1, whose place
+  // the next loads take.
+  auto enter = [&](int st) __attribute__((always_inline)) {
+    wait_stages<R, kPer>(min(R - 2, ns - 1 - st));
+    lds_barrier();
+    if (st + R - 1 < ns) issue(st + R - 1);
+  };
 
 #pragma unroll
   for (int st = 0; st < R - 1; ++st)
     if (st < ns) issue(st);
-  for (int st = 0; st < ns; ++st) {
-    wait_stages<R, kPer>(min(R - 2, ns - 1 - st));
-    lds_barrier();  // every wave's part of it; and all are done with stage st - 1, whose place the next loads take
-    if (st + R - 1 < ns) issue(st + R - 1);
-    const uint32_t xc = base + (uint32_t)(st % R) * kStage + (uint32_t)wm * (BM / WM) * RB;
-    const uint32_t wc = base + (uint32_t)(st % R) * kStage + (uint32_t)(BM + wn * (BN / WN)) * RB;
-#pragma unroll
-    for (int j = 0; j < kK; ++j) {
-      v4i xf[kFm], wf[kFn];
-#pragma unroll
-      for (int f = 0; f < kFn; ++f) wf[f] = lds_read_frag<v4i>(wc + f * 16 * RB + off[j]);
-#pragma unroll
-      for (int i = 0; i < kFm; ++i) xf[i] = lds_read_frag<v4i>(xc + i * 16 * RB + off[j]);
-#pragma unroll
-      for (int i = 0; i < kFm; ++i)
-#pragma unroll
-        for (int f = 0; f < kFn; ++f) acc[i][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f], xf[i], acc[i][f], 0, 0, 0);
+  if constexpr (kK == 1) {
+    for (int st = 0; st < ns; st += 2) {
+      enter(st);
+      read(st, 0, x0, w0);
+      multiply(x1, w1);
+      interleave();
+      __builtin_amdgcn_sched_barrier(0);
+      if (st + 1 < ns) {
+        enter(st + 1);
+        read(st + 1, 0, x1, w1);
+        multiply(x0, w0);
+        interleave();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    // The stage's reads are complete before the next stage's barrier is reached.
-    __builtin_amdgcn_sched_barrier(0);
+    if (ns % 2) multiply(x0, w0);
+    else multiply(x1, w1);
+  } else {
+    static_assert(kK % 2 == 0, "an even number of steps leaves the last in the second set");
+    for (int st = 0; st < ns; ++st) {
+      enter(st);
+#pragma unroll
+      for (int j = 0; j < kK; j += 2) {
+        read(st, j, x0, w0);
+        multiply(x1, w1);
+        interleave();
+        read(st, j + 1, x1, w1);
+        multiply(x0, w0);
+        interleave();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    multiply(x1, w1);
   }
 #pragma unroll
   for (int i = 0; i < kFm; ++i)
 #pragma unroll
     for (int f = 0; f < kFn; ++f)
       store4<T>(a, acc[i][f], split, tm * BM + wm * (BM / WM) + 16 * i + r16, tn * BN + wn * (BN / WN) + 16 * f + 4 * g);
+}
+
+// The same for many rows: 256 x 256 outputs of eight waves, 128 rows of x by 64
+// of w each, whose operands of a step of 64 k do not fit the registers twice
+// beside 128 accumulators. They are read in halves instead: while the first
+// four groups of x's rows are multiplied the other four are read, and while
+// those are, the next step's w and first half of x. RB: bytes of k a stage.
+template <typename T, int RB, int R>
+__global__ __launch_bounds__(512) void wide_gemm(GemmArgs a) {
+  constexpr int BM = 256, BN = 256, kWaves = 8;
+  constexpr int kCh = RB / 16, kRows = 64 / kCh;
+  constexpr int kPer = (BM + BN) / kRows / kWaves;
+  constexpr int kK = RB / 64;
+  constexpr int kStage = (BM + BN) * RB;
+  __shared__ __attribute__((aligned(1024))) char ring[R][kStage];
+  const int lane = (int)(threadIdx.x & 63);
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int r16 = lane & 15, g = lane >> 4;
+  const int2 tile = tile_of(a, 1);
+  const int tm = tile.x, tn = tile.y;
+  // An even number of steps: x's codes are zero up to a multiple of kPadK.
+  const int ns = (a.k + 127) / 128 * (128 / RB);
+
+  const char* src[kPer];
+  int col[kPer], cap[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int row = kRows * (wv * kPer + i) + lane / kCh;
+    col[i] = 16 * ((lane % kCh) ^ swizzle<RB>(row));
+    src[i] = row < BM ? a.x + (int64_t)min(tm * BM + row, a.m - 1) * a.x_s
+                      : a.w + (int64_t)min(tn * BN + row - BM, a.n - 1) * a.w_s;
+    cap[i] = row < BM ? 0x7fffffff : (a.k + 15) / 16 * 16 - 16;
+  }
+  const uint32_t base = lds_addr(&ring[0][0]);
+  auto issue = [&](int st) __attribute__((always_inline)) {
+    const uint32_t dst = base + (uint32_t)(st % R) * kStage + (uint32_t)wv * kPer * 1024;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) dma16<false>(src[i] + min(col[i] + st * RB, cap[i]), dst + 1024 * i);
+  };
+
+  v4i acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  const int wm = wv % 2, wn = wv / 2;
+  uint32_t xoff[kK], woff[kK];
+#pragma unroll
+  for (int j = 0; j < kK; ++j) {
+    const uint32_t o = base + (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ swizzle<RB>(r16)));
+    xoff[j] = o + (uint32_t)wm * 128 * RB;
+    woff[j] = o + (uint32_t)(BM + wn * 64) * RB;
+  }
+  v4i x0[4], x1[4], w0[4], w1[4];
+  // Groups of rows 4 h .. of x, and all four of w, of step j of the stage at `at`.
+  auto read_x = [&](uint32_t at, int j, int h, v4i (&f)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = lds_read_frag<v4i>(xoff[j] + at + (4 * h + i) * 16 * RB);
+  };
+  auto read_w = [&](uint32_t at, int j, v4i (&f)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = lds_read_frag<v4i>(woff[j] + at + i * 16 * RB);
+  };
+  auto multiply = [&](int h, const v4i (&xf)[4], const v4i (&wf)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+        acc[4 * h + i][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f], xf[i], acc[4 * h + i][f], 0, 0, 0);
+  };
+  auto spread = [&](auto reads) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < decltype(reads)::value; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 16 / decltype(reads)::value, 0);
+    }
+  };
+  auto enter = [&](int st) __attribute__((always_inline)) {
+    wait_stages<R, kPer>(min(R - 2, ns - 1 - st));
+    lds_barrier();
+    if (st + R - 1 < ns) issue(st + R - 1);
+  };
+  using Four = std::integral_constant<int, 4>;
+  using Eight = std::integral_constant<int, 8>;
+  // One step, w and the first half of x in (xa, wa); leaves the next step's in
+  // (xa, wb): of the same stage, or of stage `next`, entered first. (Past the
+  // last stage nothing is waited for and what is read is not used: without a
+  // branch here the accumulators stay where they are.)
+  auto step = [&](uint32_t at, int j, int next, int next_j, v4i (&xa)[4], v4i (&xb)[4], v4i (&wa)[4],
+                  v4i (&wb)[4]) __attribute__((always_inline)) {
+    read_x(at, j, 1, xb);
+    multiply(0, xa, wa);
+    spread(Four{});
+    __builtin_amdgcn_sched_barrier(0);
+    if (next_j == 0) enter(next);
+    const uint32_t to = next_j == 0 ? (uint32_t)(next % R) * kStage : at;
+    read_w(to, next_j, wb);
+    read_x(to, next_j, 0, xa);
+    multiply(1, xb, wa);
+    spread(Eight{});
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+#pragma unroll
+  for (int st = 0; st < R - 1; ++st)
+    if (st < ns) issue(st);
+  enter(0);
+  read_w(0, 0, w0);
+  read_x(0, 0, 0, x0);
+  if constexpr (kK == 1) {
+    for (int st = 0; st < ns; st += 2) {
+      step((uint32_t)(st % R) * kStage, 0, st + 1, 0, x0, x1, w0, w1);
+      step((uint32_t)((st + 1) % R) * kStage, 0, st + 2, 0, x0, x1, w1, w0);
+    }
+  } else {
+    static_assert(kK == 2, "two steps a stage");
+    for (int st = 0; st < ns; ++st) {
+      const uint32_t at = (uint32_t)(st % R) * kStage;
+      step(at, 0, st, 1, x0, x1, w0, w1);
+      step(at, 1, st + 1, 0, x0, x1, w1, w0);
+    }
+  }
+  const int m0 = tm * BM + wm * 128, n0 = tn * BN + wn * 64;
+  if constexpr (sizeof(T) == 2) {
+    if (a.rows16 && n0 + 64 <= a.n) {
+      // A lane holds four neighbours of a row, 16 rows to an instruction: stored
+      // as they are every store would write 32-byte pieces (the stores alone
+      // took a quarter of the call). Each wave turns its 128 rows of 128 bytes
+      // in its own part of the ring instead, chunk c of row r at c ^ r % 8, and
+      // stores whole rows.
+      static_assert(R * kStage >= 8 * 128 * 128, "the ring holds the waves' rows");
+      lds_barrier();  // every wave has read its last operands
+      const uint32_t mine = base + (uint32_t)wv * (128 * 128);
+      floatx4_t ws[4];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[f][r] = a.ws[n0 + 16 * f + 4 * g + r];
+      }
+      typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 16 * i + r16;
+        const float sx = a.xs[min(m0 + row, a.m - 1)];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][f][r] * sx * ws[f][r];
+          const int c = 2 * f + (g >> 1);
+          *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
+              (uintptr_t)(mine + row * 128 + 16 * (c ^ (row & 7)) + 8 * (g & 1))) =
+              u32x2_t{li_pack2<T>(v[0], v[1]), li_pack2<T>(v[2], v[3])};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int row = 8 * i + lane / 8, c = lane % 8;
+        const u32x4_t v = lds_read_frag<u32x4_t>(mine + row * 128 + 16 * (c ^ (row & 7)));
+        if (m0 + row < a.m)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(a.out + ((int64_t)(m0 + row) * a.o_s + n0 + 8 * c) * 2));
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) store4<T>(a, acc[i][f], 0, m0 + 16 * i + r16, n0 + 16 * f + 4 * g);
 }
 
 // out = the splits' sums, scaled and rounded.
@@ -367,7 +598,13 @@ void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
     case kFew: launch_ring<T, 16, 64, 1, 4, 256, 5>(a, s); break;
     case kSome: launch_ring<T, 64, 64, 2, 2, 256, 4>(a, s); break;
     case kMany: launch_ring<T, 128, 128, 2, 2, 128, 4>(a, s); break;
-    case kMost: launch_ring<T, 256, 256, 2, 4, 64, 4>(a, s); break;
+    case kMost: {
+      GemmArgs b = a;
+      b.mt = cdiv(a.m, 256);
+      b.nt = cdiv(a.n, 256);
+      hipLaunchKernelGGL((wide_gemm<T, 128, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(512), 0, s, b);
+      break;
+    }
   }
   if (a.splits > 1) {
     const int64_t work = (int64_t)a.m * ((a.n + 3) / 4);
@@ -439,6 +676,7 @@ extern "C" int li_linear_int8(const void* x, int64_t x_stride, const void* w, in
   a.k = k;
   a.splits = p.splits;
   a.vec = n % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0;
+  a.rows16 = out_stride % 8 == 0 && li::aligned16(out);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == LI_F32) launch_gemm<float>(a, p.kind, s);
   else if (dtype == LI_F16) launch_gemm<li_f16>(a, p.kind, s);
