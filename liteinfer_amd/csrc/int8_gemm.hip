@@ -191,14 +191,19 @@ __device__ __forceinline__ void wait_stages(int newer) {
 }
 
 // This work-group's tile: {tile of x's rows x runs + run, tile of w's rows}.
-// Work-group i runs on XCD i % 8; each XCD takes a run of tiles, side by side
-// along x's rows first, so that its L2 serves a tile of w to several.
+// Work-group i runs on XCD i % 8; each XCD takes a run of tiles in columns of
+// `kColumn` along x's rows, so that the 32 it works on at a time read few
+// rows of either operand (4 x 8 tiles: 12 rows of tiles, where 17 x 2 read
+// 19), all of them at about the same k, from its L2.
+constexpr int kColumn = 4;
 __device__ __forceinline__ int2 tile_of(const GemmArgs& a, int splits) {
   const int across = a.mt * splits, total = across * a.nt;
   const int per = total / 8, rest = total % 8;
   const int xcd = (int)(blockIdx.x % 8u), at = (int)(blockIdx.x / 8u);
   const int t = xcd * per + min(xcd, rest) + at;
-  return int2{t % across, t / across};
+  const int column = t / (kColumn * a.nt), in = t - column * kColumn * a.nt;
+  const int wide = min(kColumn, across - column * kColumn);
+  return int2{column * kColumn + in % wide, in / wide};
 }
 
 // A work-group of WM x WN waves takes BM rows of x by BN rows of w and a run
@@ -592,8 +597,25 @@ void launch_ring(GemmArgs a, hipStream_t s) {
   hipLaunchKernelGGL((ring_gemm<T, BM, BN, WM, WN, RB, R>), grid, block, 0, s, a);
 }
 
+// The rows past the last whole tile of 256, where they are few, run beside
+// the others as a product of their own: a last row of tiles costs its share
+// of a round of the GPU whatever it holds.
+constexpr int kFewLeft = 64;
+
 template <typename T>
 void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
+  const int left = a.m % 256;
+  if (kind == kMost && left && left <= kFewLeft) {
+    GemmArgs whole = a, rest = a;
+    whole.m = a.m - left;
+    launch_gemm<T>(whole, kMost, s);
+    rest.x += (int64_t)whole.m * a.x_s;
+    rest.xs += whole.m;
+    rest.out += (int64_t)whole.m * a.o_s * (int64_t)sizeof(T);
+    rest.m = left;
+    launch_gemm<T>(rest, left <= 16 ? kFew : kSome, s);
+    return;
+  }
   switch (kind) {
     case kFew: launch_ring<T, 16, 64, 1, 4, 256, 5>(a, s); break;
     case kSome: launch_ring<T, 64, 64, 2, 2, 256, 4>(a, s); break;
