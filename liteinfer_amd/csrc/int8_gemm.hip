@@ -346,19 +346,39 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
       store4<T>(a, acc[i][f], split, tm * BM + wm * (BM / WM) + 16 * i + r16, tn * BN + wn * (BN / WN) + 16 * f + 4 * g);
 }
 
-// The same for many rows: 256 x 256 outputs of eight waves, 128 rows of x by 64
-// of w each, whose operands of a step of 64 k do not fit the registers twice
-// beside 128 accumulators. They are read in halves instead: while the first
-// four groups of x's rows are multiplied the other four are read, and while
-// those are, the next step's w and first half of x. RB: bytes of k a stage.
+// acc += w x^T in place. (As a builtin the accumulators of a wave that has 256
+// of them were moved about: a thousand moves between registers in the loop.)
+__device__ __forceinline__ void add_product(v4i& acc, const v4i& w, const v4i& x) {
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+}
+// The products are complete: an accumulator may be read.
+__device__ __forceinline__ void settle(v4i (&acc)[8][8]) {
+  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[7][0]), "+a"(acc[7][1]), "+a"(acc[7][2]), "+a"(acc[7][3]),
+               "+a"(acc[7][4]), "+a"(acc[7][5]), "+a"(acc[7][6]), "+a"(acc[7][7]));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The same for many rows: 256 x 256 outputs of four waves, 128 x 128 each,
+// one wave a SIMD with its 256 accumulators in the accumulation registers and
+// two steps' operands (64 k) in the others. (Eight waves of 128 x 64 read
+// half as much again from LDS, which with the loads' writes was as busy as
+// the matrix units: 472 us for the whole call at the size below, now 435.) A step is eight groups of
+// eight products; the first four read the next step's operands, and each
+// group issues its part of the loads of the stage R - 1 ahead. RB: bytes of k
+// a stage (64 and a ring of five instead of 128 and two: whole lines of the
+// L2 are asked for twice, 480 us against 440).
+// Bound by the matrix units at the clock they leave: 4096 x 4096 by 28672 in
+// 430 us, 2.2 P operations a second, products 51% of the cycles at 1.87 GHz
+// (the same product's int32 sums alone take the library 529 us); the rest is
+// the wait for a stage (1.6 us for 1.1 us of products) and, once a tile, the
+// first stage and the store.
 template <typename T, int RB, int R>
-__global__ __launch_bounds__(512) void wide_gemm(GemmArgs a) {
-  constexpr int BM = 256, BN = 256, kWaves = 8;
-  constexpr int kCh = RB / 16, kRows = 64 / kCh;
-  constexpr int kPer = (BM + BN) / kRows / kWaves;
+__global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
+  constexpr int kRows = 1024 / RB, kPer = 512 / kRows / 4;  // rows a load, loads a wave and stage
   constexpr int kK = RB / 64;
-  constexpr int kStage = (BM + BN) * RB;
-  __shared__ __attribute__((aligned(1024))) char ring[R][kStage];
+  constexpr uint32_t kStage = 512 * RB;
+  static_assert(kPer % 8 == 0 && kPer <= 64 && (kK == 1 || kK == 2), "whole loads a group of products");
+  __shared__ __attribute__((aligned(1024))) char ring[R * kStage];
   const int lane = (int)(threadIdx.x & 63);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r16 = lane & 15, g = lane >> 4;
@@ -367,119 +387,110 @@ __global__ __launch_bounds__(512) void wide_gemm(GemmArgs a) {
   // An even number of steps: x's codes are zero up to a multiple of kPadK.
   const int ns = (a.k + 127) / 128 * (128 / RB);
 
-  const char* src[kPer];
-  int col[kPer], cap[kPer];
+  // Waves 0 and 1 bring x's rows, 2 and 3 w's; rows past the last repeat it,
+  // and w's rows end at their last chunk.
+  const bool of_x = wv < 2;
+  const int64_t stride = of_x ? a.x_s : a.w_s;
+  const int first = (of_x ? tm : tn) * 256, last = (of_x ? a.m : a.n) - 1;
+  const char* src = (of_x ? a.x : a.w) + first * stride;
+  const int cap = of_x ? 0x7fffffff : (a.k + 15) / 16 * 16 - 16;
+  uint32_t row_at[kPer];
+  int col[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int row = kRows * (wv * kPer + i) + lane / kCh;
-    col[i] = 16 * ((lane % kCh) ^ swizzle<RB>(row));
-    src[i] = row < BM ? a.x + (int64_t)min(tm * BM + row, a.m - 1) * a.x_s
-                      : a.w + (int64_t)min(tn * BN + row - BM, a.n - 1) * a.w_s;
-    cap[i] = row < BM ? 0x7fffffff : (a.k + 15) / 16 * 16 - 16;
+    const int row = 128 * (wv & 1) + kRows * i + lane / (RB / 16);
+    row_at[i] = (uint32_t)min(row, last - first) * (uint32_t)stride;
+    col[i] = 16 * ((lane % (RB / 16)) ^ swizzle<RB>(row));
   }
-  const uint32_t base = lds_addr(&ring[0][0]);
-  auto issue = [&](int st) __attribute__((always_inline)) {
-    const uint32_t dst = base + (uint32_t)(st % R) * kStage + (uint32_t)wv * kPer * 1024;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) dma16<false>(src[i] + min(col[i] + st * RB, cap[i]), dst + 1024 * i);
+  const uint32_t base = lds_addr(&ring[0]);
+  const uint32_t mine = base + (uint32_t)wv * 128 * RB;
+  auto load = [&](int st, uint32_t to, int i) __attribute__((always_inline)) {
+    dma16_at(src, row_at[i] + (uint32_t)min(col[i] + st * RB, cap), mine + to + 1024 * i);
   };
 
-  v4i acc[8][4];
+  v4i acc[8][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-  const int wm = wv % 2, wn = wv / 2;
+    for (int j = 0; j < 8; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  const int wm = wv & 1, wn = wv >> 1;
   uint32_t xoff[kK], woff[kK];
 #pragma unroll
   for (int j = 0; j < kK; ++j) {
     const uint32_t o = base + (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ swizzle<RB>(r16)));
     xoff[j] = o + (uint32_t)wm * 128 * RB;
-    woff[j] = o + (uint32_t)(BM + wn * 64) * RB;
+    woff[j] = o + (uint32_t)(256 + wn * 128) * RB;
   }
-  v4i x0[4], x1[4], w0[4], w1[4];
-  // Groups of rows 4 h .. of x, and all four of w, of step j of the stage at `at`.
-  auto read_x = [&](uint32_t at, int j, int h, v4i (&f)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = lds_read_frag<v4i>(xoff[j] + at + (4 * h + i) * 16 * RB);
-  };
-  auto read_w = [&](uint32_t at, int j, v4i (&f)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = lds_read_frag<v4i>(woff[j] + at + i * 16 * RB);
-  };
-  auto multiply = [&](int h, const v4i (&xf)[4], const v4i (&wf)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-        acc[4 * h + i][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[f], xf[i], acc[4 * h + i][f], 0, 0, 0);
-  };
-  auto spread = [&](auto reads) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < decltype(reads)::value; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 16 / decltype(reads)::value, 0);
-    }
-  };
-  auto enter = [&](int st) __attribute__((always_inline)) {
-    wait_stages<R, kPer>(min(R - 2, ns - 1 - st));
+  v4i x0[8], x1[8], w0[8], w1[8];
+  uint32_t here = 0, fill = (R - 1) * kStage;  // the ring's stage that is read from, and the one to load into
+  // Stage st is here (all of it, once every wave has come), and the one before it is free.
+  auto enter = [&]() __attribute__((always_inline)) {
+    here = here == (R - 1) * kStage ? 0 : here + kStage;
+    fill = fill == (R - 1) * kStage ? 0 : fill + kStage;
+    li_wait_vm<(R - 2) * kPer>();
     lds_barrier();
-    if (st + R - 1 < ns) issue(st + R - 1);
   };
-  using Four = std::integral_constant<int, 4>;
-  using Eight = std::integral_constant<int, 8>;
-  // One step, w and the first half of x in (xa, wa); leaves the next step's in
-  // (xa, wb): of the same stage, or of stage `next`, entered first. (Past the
-  // last stage nothing is waited for and what is read is not used: without a
-  // branch here the accumulators stay where they are.)
-  auto step = [&](uint32_t at, int j, int next, int next_j, v4i (&xa)[4], v4i (&xb)[4], v4i (&wa)[4],
-                  v4i (&wb)[4]) __attribute__((always_inline)) {
-    read_x(at, j, 1, xb);
-    multiply(0, xa, wa);
-    spread(Four{});
-    __builtin_amdgcn_sched_barrier(0);
-    if (next_j == 0) enter(next);
-    const uint32_t to = next_j == 0 ? (uint32_t)(next % R) * kStage : at;
-    read_w(to, next_j, wb);
-    read_x(to, next_j, 0, xa);
-    multiply(1, xb, wa);
-    spread(Eight{});
-    __builtin_amdgcn_sched_barrier(0);
+  // One step, its operands in (xa, wa); leaves the next step's in (xb, wb): of
+  // the same stage, or of stage `st`, entered first. (Past the last stage the
+  // last is loaded once more and what is read is not used: without branches
+  // the accumulators stay where they are.)
+  auto step = [&](int st, int j, const v4i (&xa)[8], const v4i (&wa)[8], v4i (&xb)[8], v4i (&wb)[8])
+      __attribute__((always_inline)) {
+    const bool entered = j == 0;
+    if (entered) enter();
+    const int ahead = min(st + R - 1, ns - 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        if (entered && f < kPer / 8) load(ahead, fill, i * (kPer / 8) + f);
+        const int r = (8 * i + f) / 2;
+        if (f % 2 == 0 && r < 8) wb[r] = lds_read_frag<v4i>(woff[j] + here + r * 16 * RB);
+        else if (f % 2 == 0 && r < 16) xb[r - 8] = lds_read_frag<v4i>(xoff[j] + here + (r - 8) * 16 * RB);
+        add_product(acc[i][f], wa[f], xa[i]);
+        if (f % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   };
 
 #pragma unroll
-  for (int st = 0; st < R - 1; ++st)
-    if (st < ns) issue(st);
-  enter(0);
-  read_w(0, 0, w0);
-  read_x(0, 0, 0, x0);
+  for (int st = 0; st < R; ++st)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) load(min(st, ns - 1), (uint32_t)st * kStage, i);
+  li_wait_vm<(R - 1) * kPer>();
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w0[i] = lds_read_frag<v4i>(woff[0] + i * 16 * RB);
+    x0[i] = lds_read_frag<v4i>(xoff[0] + i * 16 * RB);
+  }
   if constexpr (kK == 1) {
     for (int st = 0; st < ns; st += 2) {
-      step((uint32_t)(st % R) * kStage, 0, st + 1, 0, x0, x1, w0, w1);
-      step((uint32_t)((st + 1) % R) * kStage, 0, st + 2, 0, x0, x1, w1, w0);
+      step(st + 1, 0, x0, w0, x1, w1);
+      step(st + 2, 0, x1, w1, x0, w0);
     }
   } else {
-    static_assert(kK == 2, "two steps a stage");
     for (int st = 0; st < ns; ++st) {
-      const uint32_t at = (uint32_t)(st % R) * kStage;
-      step(at, 0, st, 1, x0, x1, w0, w1);
-      step(at, 1, st + 1, 0, x0, x1, w1, w0);
+      step(st, kK - 1, x0, w0, x1, w1);
+      step(st + 1, 0, x1, w1, x0, w0);
     }
   }
-  const int m0 = tm * BM + wm * 128, n0 = tn * BN + wn * 64;
+  settle(acc);
+  li_wait_vm<0>();
+  lds_barrier();  // every load is in and every wave has read its last operands: the ring is free
+  const int m0 = tm * 256 + wm * 128, n0 = tn * 256 + wn * 128;
   if constexpr (sizeof(T) == 2) {
-    if (a.rows16 && n0 + 64 <= a.n) {
+    if (a.rows16 && n0 + 128 <= a.n) {
       // A lane holds four neighbours of a row, 16 rows to an instruction: stored
       // as they are every store would write 32-byte pieces (the stores alone
-      // took a quarter of the call). Each wave turns its 128 rows of 128 bytes
-      // in its own part of the ring instead, chunk c of row r at c ^ r % 8, and
+      // took a quarter of the call). Each wave turns its 128 rows of 256 bytes
+      // in its own part of the ring instead, chunk c of row r at c ^ r % 16, and
       // stores whole rows.
-      static_assert(R * kStage >= 8 * 128 * 128, "the ring holds the waves' rows");
-      lds_barrier();  // every wave has read its last operands
-      const uint32_t mine = base + (uint32_t)wv * (128 * 128);
-      floatx4_t ws[4];
+      static_assert(R * kStage >= 4 * 128 * 256, "the ring holds the waves' rows");
+      const uint32_t rows = base + (uint32_t)wv * (128 * 256);
+      floatx4_t ws[8];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
+      for (int f = 0; f < 8; ++f) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) ws[f][r] = a.ws[n0 + 16 * f + 4 * g + r];
       }
@@ -489,20 +500,21 @@ __global__ __launch_bounds__(512) void wide_gemm(GemmArgs a) {
         const int row = 16 * i + r16;
         const float sx = a.xs[min(m0 + row, a.m - 1)];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
+        for (int f = 0; f < 8; ++f) {
           float v[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][f][r] * sx * ws[f][r];
           const int c = 2 * f + (g >> 1);
           *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
-              (uintptr_t)(mine + row * 128 + 16 * (c ^ (row & 7)) + 8 * (g & 1))) =
+              (uintptr_t)(rows + row * 256 + 16 * (c ^ r16) + 8 * (g & 1))) =
               u32x2_t{li_pack2<T>(v[0], v[1]), li_pack2<T>(v[2], v[3])};
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int row = 8 * i + lane / 8, c = lane % 8;
-        const u32x4_t v = lds_read_frag<u32x4_t>(mine + row * 128 + 16 * (c ^ (row & 7)));
+      for (int i = 0; i < 32; ++i) {
+        const int row = 4 * i + g, c = r16;
+        const u32x4_t v = lds_read_frag<u32x4_t>(rows + row * 256 + 16 * (c ^ (row & 15)));
         if (m0 + row < a.m)
           __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(a.out + ((int64_t)(m0 + row) * a.o_s + n0 + 8 * c) * 2));
       }
@@ -512,7 +524,10 @@ __global__ __launch_bounds__(512) void wide_gemm(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int f = 0; f < 4; ++f) store4<T>(a, acc[i][f], 0, m0 + 16 * i + r16, n0 + 16 * f + 4 * g);
+    for (int f = 0; f < 8; ++f) {
+      store4<T>(a, acc[i][f], 0, m0 + 16 * i + r16, n0 + 16 * f + 4 * g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // out = the splits' sums, scaled and rounded.
@@ -624,7 +639,7 @@ void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
       GemmArgs b = a;
       b.mt = cdiv(a.m, 256);
       b.nt = cdiv(a.n, 256);
-      hipLaunchKernelGGL((wide_gemm<T, 128, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(512), 0, s, b);
+      hipLaunchKernelGGL((wide_gemm<T, 128, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(256), 0, s, b);
       break;
     }
   }

@@ -224,6 +224,20 @@ __device__ __forceinline__ void dma4(const void* g, uint32_t lds) {
       : "memory");
 }
 
+// 64 x 16 bytes, lane i's from `at` bytes past `g` (the same in every lane) to
+// lds + 16 i.
+__device__ __forceinline__ void dma16_at(const void* g, uint32_t at, uint32_t lds) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(g)
+      : "memory");
+}
+
 // A work-group barrier that orders LDS only: this wave's LDS operations are
 // complete when it arrives, and nothing waits for its global loads or
 // stores (__syncthreads' release fence would wait for every one of them).
