@@ -450,8 +450,9 @@ int li_paged_prefill_ex(const void* q, int64_t q_stride_tok, int64_t q_stride_he
  * LI_F32, LI_F16 or LI_BF16, any head_dim up to 512 and any grouping. The
  * decode's workspace is what li_paged_decode_plan reports. The packed pass
  * needs what li_paged_prefill_int8_plan reports: it lays the chunks'
- * contexts out in `dtype` once (each value rounded to it), which the pass's
- * query blocks then share; context_tokens, the same in both calls, is the sum
+ * contexts out in fp16 once (K and V divided by a power of two for each
+ * sequence and head that keeps them in its range, each value then rounded),
+ * which the pass's query blocks then share; context_tokens, the same in both calls, is the sum
  * of context_lens where the caller knows it (0: batch x max_context), and a
  * sum below the truth leaves the rows past it unspecified. No counterpart in
  * the reference, whose roadmap (docs/roadmap.md, section 2.5) plans a

@@ -68,9 +68,11 @@ struct AttnArgs {
   float k_scale, v_scale;
   // int8 pools: kp / vp hold codes, one byte per element (pool strides in
   // bytes), slot s of KV head h standing for code * ks[s / block_size * sc_s
-  // + h] (vs for V). In a packed pass's chunks (kp / vp then a copy in the
-  // query's dtype) the flag says what its one-query rows read.
+  // + h] (vs for V). In a packed pass's chunks kp / vp are then the contexts'
+  // fp16 copy, `units` the powers of two its K and V of [batch, num_kv_heads]
+  // were divided by; its one-query rows read the codes.
   int kv_int8;
+  const float2* units;
   const float* ks;
   const float* vs;
   int64_t sc_s;
@@ -226,15 +228,18 @@ int launch_prefill_mfma(const AttnArgs& a, int dtype, hipStream_t s);
 int launch_prefill_with_rows(const AttnArgs& a, const AttnArgs& d, int dtype, hipStream_t s);
 // The combine of the balanced split's pieces (decode_mfma.hip).
 int launch_combine_balanced(const AttnArgs& d, int dtype, hipStream_t s);
-// An int8 pool's contexts in the query's dtype, for the MFMA prefill of a
-// packed pass (int8_contexts.hip): sequence after sequence, those of no query
-// left out, and those of one query too if `rows_elsewhere`. Row r of keys /
-// values [capacity, num_kv_heads, head_dim], table [batch, a.max_context]
-// naming each position's row; rows past `capacity` are left out (their
-// positions name row 0).
+// An int8 pool's contexts in fp16, for the MFMA prefill of a packed pass
+// (int8_contexts.hip): sequence after sequence, those of no query left out,
+// and those of one query too if `rows_elsewhere`. Row r of keys / values
+// [capacity, num_kv_heads, head_dim], table [batch, a.max_context] naming
+// each position's row; rows past `capacity` are left out (their positions
+// name row 0). units [batch, num_kv_heads]: what K and V were divided by
+// (written for the sequences laid out); `largest`, context_units_scratch
+// bytes, is used on the way.
 bool copy_contexts_applies(const AttnArgs& a);
-int launch_copy_contexts(const AttnArgs& a, int dtype, bool rows_elsewhere, int64_t capacity, void* keys, void* values,
-                         int64_t* table, hipStream_t s);
+size_t context_units_scratch(int batch, int num_kv_heads, int max_context);
+int launch_copy_contexts(const AttnArgs& a, bool rows_elsewhere, int64_t capacity, void* keys, void* values,
+                         int64_t* table, float2* units, uint32_t* largest, hipStream_t s);
 // Entries of the MFMA prefill work list for a pass over a slot table
 // max_context wide: an upper bound on its query blocks.
 size_t prefill_work_entries(int batch, int max_context);

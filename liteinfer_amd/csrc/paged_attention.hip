@@ -578,7 +578,7 @@ extern "C" int li_prefill_row_groups(unsigned long long row_keys, unsigned long 
 // names their rows.
 struct ContextCopy {
   int64_t rows = 0;
-  size_t table = 0, keys = 0, values = 0, need = 0;
+  size_t table = 0, keys = 0, values = 0, units = 0, largest = 0, need = 0;
 };
 ContextCopy context_copy(int batch, int num_heads, int num_kv_heads, int head_dim, int max_context, int max_query_len,
                          int64_t context_tokens) {
@@ -590,7 +590,9 @@ ContextCopy context_copy(int batch, int num_heads, int num_kv_heads, int head_di
                                        num_kv_heads, max_context));
   c.keys = c.table + (c.rows ? align256((size_t)batch * std::max(max_context, 1) * sizeof(int64_t)) : 0);
   c.values = c.keys + bytes;
-  c.need = c.values + bytes;
+  c.units = c.values + bytes;
+  c.largest = c.units + align256((size_t)batch * num_kv_heads * sizeof(float2));
+  c.need = c.largest + align256(context_units_scratch(batch, num_kv_heads, max_context));
   return c;
 }
 
@@ -644,8 +646,8 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
   if (scales) set_block_scales(a, *scales);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
-  // An int8 pool's one-query rows read the codes; its chunks read a copy of
-  // their contexts in the query's dtype.
+  // An int8 pool's one-query rows read the codes; its chunks read an fp16
+  // copy of their contexts.
   const AttnArgs rows_of = a;
   ContextCopy copy;
   bool mfma = !(flags & LI_FLAG_FORCE_GENERIC);
@@ -667,13 +669,15 @@ int paged_prefill_impl(const void* q, int64_t q_stride_tok, int64_t q_stride_hea
       a.st_s = max_context;
       a.p_s0 = (int64_t)num_kv_heads * head_dim;
       a.p_s1 = head_dim;
+      a.units = reinterpret_cast<const float2*>(wp + copy.units);
     }
   }
   mfma = mfma && prefill_mfma_applies(a, dtype);
   auto lay_out = [&](bool rows_elsewhere) -> int {
     if (!scales) return LI_OK;
-    return launch_copy_contexts(rows_of, dtype, rows_elsewhere, copy.rows, const_cast<void*>(a.kp),
-                                const_cast<void*>(a.vp), const_cast<int64_t*>(a.st), s);
+    return launch_copy_contexts(rows_of, rows_elsewhere, copy.rows, const_cast<void*>(a.kp), const_cast<void*>(a.vp),
+                                const_cast<int64_t*>(a.st), const_cast<float2*>(a.units),
+                                reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + copy.largest), s);
   };
   if (a.kv_fp8 && !mfma)
     return fail(LI_EUNSUPPORTED,

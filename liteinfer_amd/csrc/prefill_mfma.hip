@@ -752,12 +752,19 @@ struct PpLds {
   __attribute__((aligned(1024))) char vst[kPpRing][kRegion];
   int unit;
   int rows[3];  // the unit's first token + q0, its query count, first head
+  float v_unit;  // its V's power of two (an int8 pool's contexts)
   int4 entry;   // the work-list entry of `unit`
   int4 range;   // its stage range and piece ({0, all, 0, 1} for a whole block)
 };
 
 
 // LDS of a ping-pong work-group; prefill_pp_rows's row waves use it first.
+// x rounded to fp16 stays finite where x is.
+__device__ __forceinline__ float held_to_f16(float x) {
+  const bool finite = (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u;
+  return finite ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+}
+
 template <int D, int KVR>
 union PpShared {
   PpLds<D> pp;
@@ -768,13 +775,24 @@ union PpShared {
 // queue: blockIdx.x % kPrefillQueues). With kRows (prefill_pp_rows), the
 // first work-groups fold the pass's one-query rows first (the balanced
 // decode split, AttnArgs `d`, over kRowWaves waves of each of them; their
-// count was written by prefill_order), then join the queues. KVR: what the
-// rows' pool holds (int8 codes, or the type of the pool that the chunks read).
-template <typename T, int D, bool kRows, bool kSplit, bool kDirect = false, int KVR = kPool16>
+// count was written by prefill_order), then join the queues.
+//
+// TO: the queries' and outputs' type. Of a 16-bit pool it is K's and V's and
+// the matrix operands' too. Of an int8 pool (KVR; the rows read its codes)
+// the chunks read the contexts' fp16 copy and everything between the query's
+// load and the output's store is fp16: 11 bits of K, V and the weights where
+// bf16 operands would keep 8 (with them 101 bf16 queries over 4,096 keys were
+// off by 0.0047 of the outputs in the mean square, of which 0.0017 is the
+// output's own rounding). What keeps fp16's range wide enough are powers of two for
+// each sequence and KV head (int8_contexts.hip): the query is multiplied by
+// the one K was divided by, the output by V's.
+template <typename TO, int D, bool kRows, bool kSplit, bool kDirect = false, int KVR = kPool16>
 __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
+  constexpr bool kCopied = KVR == kPoolI8;
+  using T = std::conditional_t<kCopied, li_f16, TO>;
   __shared__ __attribute__((aligned(1024))) PpShared<D, KVR> lds;
   const unsigned wg = blockIdx.x;
-  if constexpr (kRows) fold_rows_first<T, D, KVR>(a, d, lds);
+  if constexpr (kRows) fold_rows_first<TO, D, KVR>(a, d, lds);
   constexpr int W = 8;
   using M = Mfma<T>;
   using Frag = typename M::Frag;
@@ -867,6 +885,7 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
   int first_slots[kSlotsPer];
   Frag qf[2][kSteps];
   bool have = false;
+  float v_unit = 1.f;
   auto fetch_inputs = [&](const int4& e, int u, int kbeg_, bool slots, bool queries) __attribute__((always_inline)) {
     const int seq_ = e.x / a.num_qblocks, qb_ = e.x % a.num_qblocks;
     const int nblk_ = (e.z + bq - 1) / bq;
@@ -880,19 +899,29 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
       for (int r = 0; r < kSlotsPer; ++r) first_slots[r] = (int)srow_[min(kbeg_ + tid + r * 64 * W, kend_ - 1)];
     }
     if (!queries) return;
+    float k_unit = sc;
+    if constexpr (kCopied) {
+      const float2 unit_of = a.units[(int64_t)seq_ * a.num_kv_heads + kvh_];
+      k_unit *= unit_of.x;
+      v_unit = unit_of.y;
+    }
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
       const int row = 32 * w + 16 * nb + n;
       const int ql = row / G;
       const bool real_ = row < bq * G && q0_ + ql < q1_;
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)(e.y + q0_ + ql) * a.q_s0 +
+      const TO* qrow = static_cast<const TO*>(a.q) + (int64_t)(e.y + q0_ + ql) * a.q_s0 +
                       (int64_t)(kvh_ * G + row % G) * a.q_s1 + 8 * g;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        Frag x = real_ ? *reinterpret_cast<const Frag*>(qrow + 32 * j) : Frag{};
+        using QFrag = typename Mfma<TO>::Frag;
+        QFrag x = real_ ? *reinterpret_cast<const QFrag*>(qrow + 32 * j) : QFrag{};
         u32x4_t pw;
 #pragma unroll
-        for (int u2 = 0; u2 < 4; ++u2) pw[u2] = li_pack2<T>((float)x[2 * u2] * sc, (float)x[2 * u2 + 1] * sc);
+        for (int u2 = 0; u2 < 4; ++u2) {
+          if constexpr (kCopied) pw[u2] = li_pack2<T>(held_to_f16((float)x[2 * u2] * k_unit), held_to_f16((float)x[2 * u2 + 1] * k_unit));
+          else pw[u2] = li_pack2<T>((float)x[2 * u2] * sc, (float)x[2 * u2 + 1] * sc);
+        }
         qf[nb][j] = __builtin_bit_cast(Frag, pw);
       }
     }
@@ -954,6 +983,9 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
   }
 
   fetch_inputs(entry, unit, kbeg, !have, true);
+  if constexpr (kCopied) {
+    if (tid == 0) lds.pp.v_unit = v_unit;
+  }
   // From here keys count from the unit's first (kbeg): its slots, the
   // rows' last visible keys and the stages' first keys.
   const int64_t* srow = a.st + (int64_t)seq * a.st_s + kbeg;
@@ -1284,7 +1316,8 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
         const int r = 32 * w + 16 * nb + en;
         float* orow = a.split_o + (slot * kMinRows + r) * D + 4 * eg;
 #pragma unroll
-        for (int blk = 0; blk < kBlk; ++blk) *reinterpret_cast<floatx4_t*>(orow + 16 * blk) = acc[nb][blk];
+        for (int blk = 0; blk < kBlk; ++blk)
+          *reinterpret_cast<floatx4_t*>(orow + 16 * blk) = kCopied ? acc[nb][blk] * lds.pp.v_unit : acc[nb][blk];
         if (eg == 0)
           *reinterpret_cast<float2*>(a.split_ml + (slot * kMinRows + r) * 2) = float2{m[nb], acc[nb][kBlk][0]};
       }
@@ -1311,13 +1344,13 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
     const uint32_t ebase = lds_addr(&kst[0][0]) + (uint32_t)w * (32 * L::kRowBytes);
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
-      const float inv = 1.f / acc[nb][kBlk][0];
+      const float inv = (kCopied ? lds.pp.v_unit : 1.f) / acc[nb][kBlk][0];
       const int r = 16 * nb + en;
 #pragma unroll
       for (int blk = 0; blk < kBlk; ++blk) {
         typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-        const u32x2_t wv = {li_pack2<T>(acc[nb][blk][0] * inv, acc[nb][blk][1] * inv),
-                            li_pack2<T>(acc[nb][blk][2] * inv, acc[nb][blk][3] * inv)};
+        const u32x2_t wv = {li_pack2<TO>(acc[nb][blk][0] * inv, acc[nb][blk][1] * inv),
+                            li_pack2<TO>(acc[nb][blk][2] * inv, acc[nb][blk][3] * inv)};
         const int c = 2 * blk + (eg >> 1);  // the piece: bytes 32 blk + 8 g of the row
         *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
             (uintptr_t)(ebase + r * L::kRowBytes + 16 * (c ^ (r % kCh)) + 8 * (eg & 1))) = wv;
@@ -1338,7 +1371,7 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
       const int row = 32 * w + r;
       const int ql = row / a.groups;
       if (ql < nvalid) {  // (so row < block_q * G too)
-        T* orow = static_cast<T*>(a.out) + (int64_t)(tok0 + ql) * a.o_s0 +
+        TO* orow = static_cast<TO*>(a.out) + (int64_t)(tok0 + ql) * a.o_s0 +
                   (int64_t)(head0 + row % a.groups) * a.o_s1 + 8 * c;
         *reinterpret_cast<u32x4_t*>(orow) = v;
       }
@@ -1348,9 +1381,9 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
   }  // units
 }
 
-template <typename T, int D, bool kSplit, bool kDirect>
+template <typename T, int D, bool kSplit, bool kDirect, int KVR>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefill_pp(AttnArgs a) {
-  prefill_pp_body<T, D, false, kSplit, kDirect>(a, a);
+  prefill_pp_body<T, D, false, kSplit, kDirect, KVR>(a, a);
 }
 
 // A packed pass's chunks and one-query rows in one launch: the first
@@ -1757,12 +1790,17 @@ static int launch_prefill_waves(AttnArgs a, int dtype, hipStream_t s, const Attn
       else hipLaunchKernelGGL((prefill_mfma<li_f16, 128, W, true, false>), g, block, 0, s, a);
     }
   } else {
-#define LI_PP(T, D)                                                                                 \
-  do {                                                                                              \
-    if (a.split_ok && direct) hipLaunchKernelGGL((prefill_pp<T, 64, true, true>), g, block, 0, s, a); \
-    else if (a.split_ok) hipLaunchKernelGGL((prefill_pp<T, D, true, false>), g, block, 0, s, a);    \
-    else if (direct) hipLaunchKernelGGL((prefill_pp<T, D, false, true>), g, block, 0, s, a);        \
-    else hipLaunchKernelGGL((prefill_pp<T, D, false, false>), g, block, 0, s, a);                   \
+#define LI_PP_OF(T, D, KVR)                                                                              \
+  do {                                                                                                   \
+    if (a.split_ok && direct) hipLaunchKernelGGL((prefill_pp<T, 64, true, true, KVR>), g, block, 0, s, a); \
+    else if (a.split_ok) hipLaunchKernelGGL((prefill_pp<T, D, true, false, KVR>), g, block, 0, s, a);    \
+    else if (direct) hipLaunchKernelGGL((prefill_pp<T, D, false, true, KVR>), g, block, 0, s, a);        \
+    else hipLaunchKernelGGL((prefill_pp<T, D, false, false, KVR>), g, block, 0, s, a);                   \
+  } while (0)
+#define LI_PP(T, D)                        \
+  do {                                     \
+    if (a.kv_int8) LI_PP_OF(T, D, kPoolI8); \
+    else LI_PP_OF(T, D, kPool16);          \
   } while (0)
     if (dtype == LI_BF16) {
       if (a.head_dim == 128) LI_PP(li_bf16, 128);
@@ -1772,6 +1810,7 @@ static int launch_prefill_waves(AttnArgs a, int dtype, hipStream_t s, const Attn
       else LI_PP(li_f16, 64);
     }
 #undef LI_PP
+#undef LI_PP_OF
   }
   if (int rc = check_launch("prefill_mfma")) return rc;
   return launch_prefill_merge(a, dtype, s, direct);

@@ -596,8 +596,9 @@ def paged_prefill(
         out: where to write the result (the query's shape and dtype, last
             axis contiguous, any other strides); a new tensor when None.
         key_scales, value_scales: an int8 pool's scales (see `paged_decode`).
-            The MFMA kernels then read the chunks' contexts from a copy in the
-            query's dtype that the call makes, as the dense kernels gather them.
+            The MFMA kernels then read the chunks' contexts from a copy in
+            fp16 that the call makes, whatever the query's dtype (K and V
+            each over a power of two that keeps them in its range).
         context_tokens: the sum of `context_lens` where the host knows it
             (an int8 pool's copy holds as many rows; None: batch times the
             table's width). Less than the sum leaves the result unspecified.

@@ -14,15 +14,15 @@ relative to a value (bf16 2^-8, fp16 2^-11, fp32 2^-24):
   2^-24 times 32 and log2 e, a few operations over, and D 2^-22 of the largest
   q k, below 2^-15).
 * decode and packed passes, general kernel: fp32 throughout, 2^-14 A.
-* packed passes, MFMA kernels: over K and V rounded to the query's dtype (as
-  the dense kernels gather them; the oracle is given those), weights rounded
-  to it, h(t) A, and its sum taken of the rounded weights, h(t) |out| more;
-  the query, with the softmax scale in it, is rounded to its dtype, which
-  moves a score by at most E = h(t) times scale times the largest sum of
-  |q k|, a weight by a factor within e^-E .. e^E, and with its share of the
-  sum the output by at most (e^2E - 1) (A + |out|). Loose, so beside it these
-  passes are held bit for bit to the same kernel over a 16-bit pool that
-  holds the rounded values.
+* packed passes, MFMA kernels, with h = h(fp16): K and V are rounded to fp16
+  after a division by a power of two that keeps them in its range, weights
+  are rounded to it: 2 h A and, as their sum is taken of the rounded weights,
+  h |out|; weights below its normal range as in decode. The query, with the
+  softmax scale in it, is rounded to fp16 too: with K's rounding this moves a
+  score by at most E = scale (2 h times the largest sum of |q k|, and for what
+  lies below the normal range 2^-24 times the sums of |q| and of |k|, each in
+  its unit), a weight by a factor within e^-E .. e^E, and with its share of the sum the
+  output by at most (e^2E - 1) (A + |out|).
 * and the output's rounding, h(t) |out|.
 """
 
@@ -90,30 +90,37 @@ class Batch:
                              torch.from_numpy(self.starts).to(DEV), max(self.queries), self.scaling, self.groups,
                              key_scales=ks, value_scales=vs, **kw)
 
-    def want(self, rounded=False):
-        """(attention, attention over |V|) in 64 bits; over K and V rounded to the query's dtype if `rounded`."""
+    def want(self):
+        """(attention, attention over |V|) in 64 bits."""
         keys, values = (I8.dequantize(c, s) for c, s in zip(self.codes, self.scales))
-        if rounded:
-            keys, values = (torch.from_numpy(t.astype(np.float32)).to(self.dtype).double().numpy() for t in (keys, values))
         q = self.query.double().cpu().numpy()
         return [attend(q, keys, v, self.table, np.asarray(self.contexts), self.scaling, self.groups, self.starts)
                 for v in (values, np.abs(values))]
 
-    def query_step(self):
+    def moved(self):
         """e^2E - 1 of the packed passes' bound, for each query row and head: [rows, heads, 1]."""
         keys = np.abs(I8.dequantize(self.codes[0], self.scales[0]))
         q = np.abs(self.query.double().cpu().numpy())
         most = np.stack([(q[:, h] @ keys[:, h // self.groups].T).max(axis=1) for h in range(self.heads)], axis=1)
-        return np.expm1(2 * half_step(self.dtype) * self.scaling * most)[..., None]
+        unit = 2.0 ** (np.floor(np.log2(self.scales[0].max())) + 4)  # K's; of a short context down to 2^-3 of it
+        small = 2.0 ** -24 * (q.sum(axis=2) * unit + 8 * keys.sum(axis=2).max() / unit)
+        return np.expm1(2 * self.scaling * (2 * half_step(F16) * most + small))[..., None]
 
-    def check(self, out, weight_step, rounded=False, extra=0.0):
-        want, size = self.want(rounded)
+    def check(self, out, weight_step, copied=None):
+        """`copied`: the rows that read a packed pass's copy of their contexts."""
+        want, size = self.want()
         got = out.double().cpu().numpy()
         assert out.dtype == self.dtype and got.shape == want.shape
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
-        moved = self.query_step() if rounded else 0.0
         small = max(self.contexts) * 2.0 ** -24 * np.nanmax(np.abs(I8.dequantize(self.codes[1], self.scales[1])))
-        bound = small + (weight_step + moved + 2.0 ** -14) * size + (half_step(self.dtype) + moved + extra) * np.abs(want) * (1 + 2.0 ** -7)
+        step = half_step(self.dtype)
+        extra = 0.0
+        if copied is not None:
+            of = np.asarray(copied).reshape(-1, 1, 1)
+            moved = self.moved()
+            weight_step = np.where(of, 2 * half_step(F16) + moved, weight_step)
+            extra = np.where(of, half_step(F16) + moved, 0.0)
+        bound = small + (weight_step + 2.0 ** -14) * size + (step + extra) * np.abs(want) * (1 + 2.0 ** -7)
         bad = np.abs(got - want) > bound + 1e-30
         assert not bad.any(), (np.abs(got - want)[bad].max(), (np.abs(got - want) / bound)[bad].max(), np.argwhere(bad)[:4])
 
@@ -177,35 +184,34 @@ def test_packed_passes(name, tokens, dtype):
 
 
 def _check_packed(batch, out):
-    """Rows of one query are decoded (unrounded K and V), the others read the copy in the query's dtype."""
-    step = half_step(batch.dtype)
-    rows = np.repeat(np.asarray(batch.queries) == 1, batch.queries)
-    exact, size = batch.want()
-    copied, copied_size = batch.want(rounded=True)
-    got = out.double().cpu().numpy()
-    moved = batch.query_step()
-    for want, a, weight, extra, which in ((exact, size, half_step(F16), 0.0, rows),
-                                          (copied, copied_size, step + moved, step + moved, ~rows)):
-        small = max(batch.contexts) * 2.0 ** -24 * np.abs(I8.dequantize(batch.codes[1], batch.scales[1])).max()
-        bound = small + (weight + 2.0 ** -14) * a + (step + extra) * np.abs(want) * (1 + 2.0 ** -7)
-        bad = (np.abs(got - want) > bound)[which]
-        assert not bad.any(), (np.abs(got - want)[which][bad].max(), np.argwhere(bad)[:4])
-    assert np.isfinite(got).all()
+    """Rows of one query are decoded, the others read the copy."""
+    batch.check(out, half_step(F16), copied=np.repeat(np.asarray(batch.queries) > 1, batch.queries))
+    assert torch.isfinite(out).all()
 
 
-@pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("name", PASSES)
-def test_packed_passes_read_what_a_16_bit_pool_would_hold(name, dtype):
-    batch = Batch(**PASSES[name], dtype=dtype)
-    got = batch.prefill(one_query_rows=False) if max(batch.queries) > 1 else None
-    pools = [torch.from_numpy(I8.dequantize(c, s).astype(np.float32)).to(dtype).to(DEV)
-             for c, s in zip(batch.codes, batch.scales)]
-    want = paged_prefill(batch.query, *pools, batch.table_t, batch.contexts_t, torch.from_numpy(batch.starts).to(DEV),
-                         max(batch.queries), batch.scaling, batch.groups, one_query_rows=False)
-    assert got is None or torch.equal(got, want)
-    if any(q == 1 for q in batch.queries):  # the rows beside the chunks are decoded; the chunks stay what they are
-        rows = torch.repeat_interleave(torch.tensor([q == 1 for q in batch.queries]), torch.tensor(batch.queries))
-        assert torch.equal(batch.prefill()[~rows], want[~rows])
+SPREAD = dict(contexts=[700, 90, 5000, 33], queries=[100, 1, 300, 20], heads=8, kv_heads=2, width=5000)
+
+
+@pytest.mark.parametrize("power", [-90, -30, 12, 40, 100])
+def test_packed_passes_over_values_of_any_size(power):
+    """V times a power of two: the output times it, bit for bit (the units are one for each head)."""
+    batch = Batch(**SPREAD)
+    plain = batch.prefill(one_query_rows=False)
+    batch.scales[1][:, 1] *= np.float32(2.0 ** power)
+    got = batch.prefill(one_query_rows=False)
+    assert torch.equal(got[:, :4], plain[:, :4])
+    assert torch.equal(got[:, 4:], plain[:, 4:] * 2.0 ** power)
+
+
+@pytest.mark.parametrize("power", [-80, -20, 5, 18, 60])
+def test_packed_passes_over_keys_of_any_size(power):
+    """K times a power of two and the query by its inverse: the same output, bit for bit."""
+    batch = Batch(**SPREAD)
+    plain = batch.prefill()
+    _check_packed(batch, plain)
+    batch.scales[0] *= np.float32(2.0 ** power)
+    batch.query = batch.query * 2.0 ** -power
+    assert torch.equal(batch.prefill(), plain)
 
 
 @pytest.mark.parametrize("name", PASSES)
@@ -220,7 +226,7 @@ def test_rows_folded_as_queries_of_the_pass(flag):
     batch = Batch(contexts=[300, 900, 70, 2000], queries=[100, 1, 33, 1], heads=32, kv_heads=8)
     out = batch.prefill(one_query_rows=flag)
     if flag is False:  # every sequence reads the copy
-        batch.check(out, half_step(BF16), rounded=True, extra=half_step(BF16))
+        batch.check(out, half_step(F16), copied=np.ones(sum(batch.queries), bool))
     else:
         _check_packed(batch, out)
 
@@ -324,7 +330,7 @@ def test_slots_past_32_bits_of_bytes():
     ks[-5:], vs[-5:] = (torch.from_numpy(s).to(DEV) for s in batch.scales)
     out = paged_prefill(batch.query, keys, values, batch.table_t + far, batch.contexts_t,
                         torch.from_numpy(batch.starts).to(DEV), 30, batch.scaling, 1, key_scales=ks, value_scales=vs)
-    batch.check(out, half_step(BF16), rounded=True, extra=half_step(BF16))
+    batch.check(out, half_step(F16), copied=np.ones(sum(batch.queries), bool))
 
 
 def test_strided_operands():
