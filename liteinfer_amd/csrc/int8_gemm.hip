@@ -74,7 +74,8 @@ __device__ __forceinline__ uint32_t largest_of(const Vec8<E>& x) {
 // registers between the maximum and the codes; longer rows are read twice.
 // Memory-bound.
 // ---------------------------------------------------------------------------
-constexpr int kQuantThreads = 256;
+
+constexpr int kQuantHold = 2048;
 
 // Eight values of a row from column d (zeros past k), whatever its alignment.
 template <typename E, bool kVec>
@@ -88,10 +89,10 @@ __device__ __forceinline__ Vec8<E> row_values(const E* row, int d, int k) {
   return v;
 }
 
-template <typename E, bool kVec>
+template <typename E, bool kVec, int kQuantThreads>
 __global__ __launch_bounds__(kQuantThreads) void quantize_rows(const E* x, int64_t x_s, int8_t* codes, int64_t c_s,
                                                                float* scales, int k, int padded) {
-  constexpr int kHold = 8;
+  constexpr int kHold = kQuantHold / kQuantThreads;
   const int tid = threadIdx.x;
   const E* row = x + (int64_t)blockIdx.x * x_s;
   Vec8<E> held[kHold];
@@ -346,6 +347,81 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
       store4<T>(a, acc[i][f], split, tm * BM + wm * (BM / WM) + 16 * i + r16, tn * BN + wn * (BN / WN) + 16 * f + 4 * g);
 }
 
+// Up to 16 rows: bound by the reading of w. A work-group takes 16 of w's rows,
+// each of its four waves a quarter of k with a ring of its own (no barriers;
+// XR of x's rows beside w's 16, R stages of 256 bytes a row in flight), and
+// the waves' sums meet in LDS: no second kernel joins runs of k. (Tiles of 64
+// of w's rows, k cut over the grid and a second kernel took 12.9 us a call at
+// 1 x 4096 by 6144 where this takes 9.1, quantising included, 21.4 for 14.0 at
+// 1 x 14336 by 4096, 21.8 for 15.9 with 16 rows. Operands loaded straight into
+// registers and x quantised in every work-group: 20.1, 61 and 45.) 117 MB of w
+// come at 5.6 TB/s; what is left at 25 MB is two launches and a wave's eight
+// stages. XR = 4 where it does (4 rows: 9.1, as 16: 10.5).
+template <typename T, int XR, int R>
+__global__ __launch_bounds__(256) void few_gemm(GemmArgs a) {
+  constexpr int kPer = (16 + XR) / 4;  // loads a stage, four rows each
+  constexpr uint32_t kStage = 1024 * kPer;
+  __shared__ __attribute__((aligned(1024))) char ring[4 * R * kStage];
+  const int lane = (int)(threadIdx.x & 63);
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int r16 = lane & 15, g = lane >> 4;
+  const int n0 = 16 * (int)blockIdx.x;
+  const int stages = (a.k + 255) / 256, part = (stages + 3) / 4;
+  const int s0 = wv * part, ns = min(part, stages - s0);
+  const char* src[kPer];
+  int col[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int row = (i < 4 ? 4 * i : 4 * (i - 4)) + g;
+    col[i] = 16 * (r16 ^ swizzle<256>(row)) + s0 * 256;
+    src[i] = i < 4 ? a.w + (int64_t)min(n0 + row, a.n - 1) * a.w_s : a.x + (int64_t)min(row, a.m - 1) * a.x_s;
+  }
+  const int cap = (a.k + 15) / 16 * 16 - 16;  // w's rows end at their last chunk; x's go on in zeros
+  const uint32_t base = lds_addr(&ring[0]);
+  const uint32_t mine = base + (uint32_t)wv * (R * kStage);
+  auto issue = [&](int st) __attribute__((always_inline)) {
+    const uint32_t to = mine + (uint32_t)(st % R) * kStage;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = col[i] + st * 256;
+      if (i < 4) dma16<true>(src[i] + min(at, cap), to + 1024 * i);
+      else dma16<false>(src[i] + at, to + 1024 * i);
+    }
+  };
+  uint32_t woff[4], xoff[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    woff[j] = mine + (uint32_t)(r16 * 256 + 16 * ((4 * j + g) ^ swizzle<256>(r16)));
+    xoff[j] = mine + 4096 + (uint32_t)(r16 % XR * 256 + 16 * ((4 * j + g) ^ swizzle<256>(r16 % XR)));
+  }
+  v4i acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int st = 0; st < R; ++st)
+    if (st < ns) issue(st);
+  for (int st = 0; st < ns; ++st) {
+    wait_stages<R + 1, kPer>(min(R - 1, ns - 1 - st));
+    const uint32_t at = (uint32_t)(st % R) * kStage;
+    v4i wf[4], xf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      wf[j] = lds_read_frag<v4i>(woff[j] + at);
+      xf[j] = lds_read_frag<v4i>(xoff[j] + at);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before the next loads write there
+    if (st + R < ns) issue(st + R);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], xf[j], acc, 0, 0, 0);
+  }
+  // (Every load of the wave is in: its ring is free.)
+  *reinterpret_cast<__attribute__((address_space(3))) v4i*>((uintptr_t)(mine + 16 * lane)) = acc;
+  __syncthreads();
+  if (wv) return;
+  v4i sum = {0, 0, 0, 0};
+#pragma unroll
+  for (int p = 0; p < 4; ++p) sum += lds_read_frag<v4i>(base + p * (R * kStage) + 16 * lane);
+  store4<T>(a, sum, 0, r16, n0 + 4 * g);
+}
+
 // acc += w x^T in place. (As a builtin the accumulators of a wave that has 256
 // of them were moved about: a thousand moves between registers in the loop.)
 __device__ __forceinline__ void add_product(v4i& acc, const v4i& w, const v4i& x) {
@@ -538,6 +614,7 @@ __global__ __launch_bounds__(256) void reduce_sums(GemmArgs a) {
   if (i >= a.m * quads) return;
   const int m = (int)(i / quads), n = (int)(i - m * quads) * 4;
   v4i s = {0, 0, 0, 0};
+#pragma unroll 4
   for (int p = 0; p < a.splits; ++p) {
     const int32_t* src = a.part + ((int64_t)p * a.m + m) * a.n + n;
     if (a.vec && n + 4 <= a.n) {
@@ -562,12 +639,12 @@ struct Plan {
 Plan plan_of(int m, int n, int k) {
   const int cus = li::device_cu_count();
   Plan p{};
-  if (m <= 16) p = {kFew, 16, 64, 1};
+  if (m <= 16) p = {kFew, 16, 16, 1};
   else if (m <= 64) p = {kSome, 64, 64, 1};
   else if ((int64_t)cdiv(m, 256) * cdiv(n, 256) < cus) p = {kMany, 128, 128, 1};
   else p = {kMost, 256, 256, 1};
   const int64_t tiles = (int64_t)cdiv(m, p.bm) * cdiv(n, p.bn);
-  if (tiles * 4 < cus * 3) p.splits = std::max<int>(1, std::min<int64_t>(cus / tiles, cdiv(k, 1024)));
+  if (p.kind != kFew && tiles * 4 < cus * 3) p.splits = std::max<int>(1, std::min<int64_t>(cus / tiles, cdiv(k, 1024)));
   return p;
 }
 
@@ -594,14 +671,23 @@ int check_extents(const char* who, int m, int n, int k) {
   return LI_OK;
 }
 
+// Few long rows take four times the threads each: 61 rows of 14,336 bring a
+// call from 24.6 us to 23.1, 256 of 4,096 from 23.1 to 21.5; 600 of 14,336
+// lose by it (80.5 -> 82.5), as their work-groups fill the GPU anyway.
+constexpr int kQuantWideRows = 512, kQuantWideK = 2048;
 template <typename E>
 void launch_quantize(const void* x, int64_t x_s, void* codes, int64_t c_s, float* scales, int m, int k, int padded,
                      hipStream_t s) {
   const bool vec = li::aligned16(x) && (x_s * (int64_t)sizeof(E)) % 16 == 0;
   const E* xp = static_cast<const E*>(x);
   int8_t* cp = static_cast<int8_t*>(codes);
-  if (vec) hipLaunchKernelGGL((quantize_rows<E, true>), dim3((unsigned)m), dim3(kQuantThreads), 0, s, xp, x_s, cp, c_s, scales, k, padded);
-  else hipLaunchKernelGGL((quantize_rows<E, false>), dim3((unsigned)m), dim3(kQuantThreads), 0, s, xp, x_s, cp, c_s, scales, k, padded);
+#define LI_QUANTIZE(VEC, THREADS) \
+  hipLaunchKernelGGL((quantize_rows<E, VEC, THREADS>), dim3((unsigned)m), dim3(THREADS), 0, s, xp, x_s, cp, c_s, scales, k, padded)
+  const bool wide = m < kQuantWideRows && k > kQuantWideK;
+  if (vec && wide) LI_QUANTIZE(true, 1024);
+  else if (vec) LI_QUANTIZE(true, 256);
+  else LI_QUANTIZE(false, 256);
+#undef LI_QUANTIZE
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int RB, int R>
@@ -632,7 +718,10 @@ void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
     return;
   }
   switch (kind) {
-    case kFew: launch_ring<T, 16, 64, 1, 4, 256, 5>(a, s); break;
+    case kFew:
+      if (a.m <= 4) hipLaunchKernelGGL((few_gemm<T, 4, 3>), dim3((unsigned)cdiv(a.n, 16)), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((few_gemm<T, 16, 2>), dim3((unsigned)cdiv(a.n, 16)), dim3(256), 0, s, a);
+      break;
     case kSome: launch_ring<T, 64, 64, 2, 2, 256, 4>(a, s); break;
     case kMany: launch_ring<T, 128, 128, 2, 2, 128, 4>(a, s); break;
     case kMost: {
