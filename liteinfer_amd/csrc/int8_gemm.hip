@@ -630,21 +630,43 @@ __global__ __launch_bounds__(256) void reduce_sums(GemmArgs a) {
   store4<T>(whole, s, 0, m, n);
 }
 
+// Of tiles of 256 rows the last, where it would hold few, runs after the
+// others as a product of its own: a row of tiles costs its share of a round
+// of the GPU whatever it holds (4099 x 4096 by 28672: 521 us -> 488).
+constexpr int kFewLeft = 64;
+constexpr int64_t kWideStride = int64_t(1) << 23;  // 255 rows of it and a row's bytes stay below 2^32
+
 // Which kernel a product runs on and the runs its k is cut into.
 enum Kind { kFew, kSome, kMany, kMost };
 struct Plan {
   Kind kind;
   int bm, bn, splits;
 };
+// Tiles of 64 x 64 while they fit the GPU at once: against 128 x 128 they give
+// 16 us for 20 at 100 x 4096 by 4096, 17 for 22 at 256 rows, 12 for 18 at 300 x
+// 2048 by 2048; with more of them than compute units 128 x 128 wins (52 for 40
+// at 100 x 4096 by 28672).
+// Above, a round of tiles of 256 x 256 (one a compute unit) takes as long as
+// 2.2 rounds of 128 x 128 for four times the work, so what the last round
+// leaves idle decides. Against 128 x 128: 71 us for 120 at 512 x 4096 by 28672
+// (1 round, 4), 76 for 88 at 1300 x 4096 by 6144 (1, 3), 119 for 145 at 3000
+// (2, 5), 255 for 412 at 2048 by 28672; but 85 for 67 at 2048 x 4096 by 4096
+// (1, 2), 80 for 62 at 1000 x 4096 by 6144 (1, 2).
+// Tiles that leave a quarter of the GPU idle cut k, to runs of 1,024 at least:
+// 40 us -> 24 at 64 x 14336 by 4096, 77 -> 28 at 100 rows.
 Plan plan_of(int m, int n, int k) {
   const int cus = li::device_cu_count();
+  const auto rounds = [&](int64_t tm, int64_t tn) { return (tm * tn + cus - 1) / cus; };
+  const int left = m % 256;
+  const int64_t large = rounds(left && left <= kFewLeft ? m / 256 : cdiv(m, 256), cdiv(n, 256));
   Plan p{};
   if (m <= 16) p = {kFew, 16, 16, 1};
-  else if (m <= 64) p = {kSome, 64, 64, 1};
-  else if ((int64_t)cdiv(m, 256) * cdiv(n, 256) < cus) p = {kMany, 128, 128, 1};
+  else if (m <= 64 || (int64_t)cdiv(m, 64) * cdiv(n, 64) <= cus) p = {kSome, 64, 64, 1};
+  else if (4 * rounds(cdiv(m, 128), cdiv(n, 128)) <= 9 * large) p = {kMany, 128, 128, 1};
   else p = {kMost, 256, 256, 1};
   const int64_t tiles = (int64_t)cdiv(m, p.bm) * cdiv(n, p.bn);
-  if (p.kind != kFew && tiles * 4 < cus * 3) p.splits = std::max<int>(1, std::min<int64_t>(cus / tiles, cdiv(k, 1024)));
+  if ((p.kind == kSome || p.kind == kMany) && tiles * 4 < cus * 3)
+    p.splits = std::max<int>(1, std::min<int64_t>(cus / tiles, cdiv(k, 1024)));
   return p;
 }
 
@@ -697,11 +719,6 @@ void launch_ring(GemmArgs a, hipStream_t s) {
   const dim3 grid((unsigned)(a.mt * a.nt * a.splits)), block(64 * WM * WN);
   hipLaunchKernelGGL((ring_gemm<T, BM, BN, WM, WN, RB, R>), grid, block, 0, s, a);
 }
-
-// The rows past the last whole tile of 256, where they are few, run beside
-// the others as a product of their own: a last row of tiles costs its share
-// of a round of the GPU whatever it holds.
-constexpr int kFewLeft = 64;
 
 template <typename T>
 void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
@@ -804,8 +821,10 @@ extern "C" int li_linear_int8(const void* x, int64_t x_stride, const void* w, in
   a.vec = n % 4 == 0 && out_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) % (4 * esize)) == 0;
   a.rows16 = out_stride % 8 == 0 && li::aligned16(out);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == LI_F32) launch_gemm<float>(a, p.kind, s);
-  else if (dtype == LI_F16) launch_gemm<li_f16>(a, p.kind, s);
-  else launch_gemm<li_bf16>(a, p.kind, s);
+  // (The large tiles reach their rows by 32-bit offsets.)
+  const Kind kind = p.kind == kMost && w_stride > kWideStride ? kMany : p.kind;
+  if (dtype == LI_F32) launch_gemm<float>(a, kind, s);
+  else if (dtype == LI_F16) launch_gemm<li_f16>(a, kind, s);
+  else launch_gemm<li_bf16>(a, kind, s);
   return li::check_launch("li_linear_int8");
 }

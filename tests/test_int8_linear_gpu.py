@@ -56,6 +56,26 @@ def test_sizes_of_the_engine(shape, dtype):
     _check(ops.linear_int8(x.to(DEV), *_weight(codes, scales)), x, codes, scales)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", [(530, 2051, 77), (530, 2051, 2100), (1300, 6147, 131), (1400, 6147, 131), (1283, 6148, 300),
+                                   (1290, 6152, 128)])
+def test_large_tiles_at_odd_sizes(shape, dtype):
+    """128 x 128 whole and cut along k; 256 x 256 with 20, 120, 3 and 10 rows past the last whole one."""
+    x, codes, scales = _operands(*shape, dtype)
+    _check(ops.linear_int8(x.to(DEV), *_weight(codes, scales)), x, codes, scales)
+
+
+def test_rows_of_a_weight_far_apart():
+    """A tile of 256 of w's rows spans more than 2^32 bytes."""
+    m, n, k = 1400, 6147, 131
+    x, codes, scales = _operands(m, n, k, BF16)
+    held = torch.empty(n * ((1 << 24) + 16), dtype=torch.int8, device=DEV).view(n, -1)[:, :k]
+    held.copy_(torch.from_numpy(codes).to(DEV))
+    _check(ops.linear_int8(x.to(DEV), held, torch.from_numpy(scales).to(DEV)), x, codes, scales)
+    del held
+    torch.cuda.empty_cache()
+
+
 def test_the_largest_sums():
     """Codes of one sign at the longest k: the sums come near 2^31."""
     k = 131072
