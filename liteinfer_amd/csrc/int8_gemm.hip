@@ -181,12 +181,8 @@ __device__ __forceinline__ void store4(const GemmArgs& a, const v4i& acc, int sp
 // Waits until at most `newer` stages of kPer loads each are in flight.
 template <int R, int kPer>
 __device__ __forceinline__ void wait_stages(int newer) {
-  static_assert(R >= 2 && R <= 8 && (R - 2) * kPer < 64, "vmcnt range");
-  if (R > 7 && newer >= 6) li_wait_vm<(R > 7 ? 6 * kPer : 0)>();
-  else if (R > 6 && newer >= 5) li_wait_vm<(R > 6 ? 5 * kPer : 0)>();
-  else if (R > 5 && newer >= 4) li_wait_vm<(R > 5 ? 4 * kPer : 0)>();
-  else if (R > 4 && newer >= 3) li_wait_vm<(R > 4 ? 3 * kPer : 0)>();
-  else if (R > 3 && newer >= 2) li_wait_vm<(R > 3 ? 2 * kPer : 0)>();
+  static_assert(R >= 2 && R <= 4 && (R - 2) * kPer < 64, "vmcnt range");
+  if (R > 3 && newer >= 2) li_wait_vm<(R > 3 ? 2 * kPer : 0)>();
   else if (R > 2 && newer >= 1) li_wait_vm<(R > 2 ? kPer : 0)>();
   else li_wait_vm<0>();
 }
@@ -213,14 +209,12 @@ __device__ __forceinline__ int2 tile_of(const GemmArgs& a, int splits) {
 // served 16 lanes at a time, lanes 0-3, 12-15, 20-23 and 24-27 together, then
 // 4-11, 16-19 and 28-31, then the same of the upper half: eight rows of one
 // chunk with eight others of the next, which the swizzles keep in 16 different
-// bank groups (with rows of 64 bytes swizzled by r / 4 every read took twice
-// its time). R - 1 stages are in flight, one barrier a stage; the operands of
+// bank groups. R - 1 stages are in flight, one barrier a stage; the operands of
 // one step of 64 k are read while the step before is multiplied, across the
 // barrier too, one read with every few products.
 template <int RB>
 __device__ __forceinline__ int swizzle(int row) {
-  if constexpr (RB == 64) return (0x78 >> (2 * ((row >> 2) & 3))) & 3;  // 0, 2, 3, 1
-  else return (row / (256 / RB)) % (RB / 16);
+  return (row / (256 / RB)) % (RB / 16);
 }
 template <typename T, int BM, int BN, int WM, int WN, int RB, int R>
 __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
@@ -306,40 +300,21 @@ __global__ __launch_bounds__(64 * WM * WN) void ring_gemm(GemmArgs a) {
 #pragma unroll
   for (int st = 0; st < R - 1; ++st)
     if (st < ns) issue(st);
-  if constexpr (kK == 1) {
-    for (int st = 0; st < ns; st += 2) {
-      enter(st);
-      read(st, 0, x0, w0);
+  static_assert(kK % 2 == 0, "an even number of steps leaves the last in the second set");
+  for (int st = 0; st < ns; ++st) {
+    enter(st);
+#pragma unroll
+    for (int j = 0; j < kK; j += 2) {
+      read(st, j, x0, w0);
       multiply(x1, w1);
       interleave();
-      __builtin_amdgcn_sched_barrier(0);
-      if (st + 1 < ns) {
-        enter(st + 1);
-        read(st + 1, 0, x1, w1);
-        multiply(x0, w0);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      read(st, j + 1, x1, w1);
+      multiply(x0, w0);
+      interleave();
     }
-    if (ns % 2) multiply(x0, w0);
-    else multiply(x1, w1);
-  } else {
-    static_assert(kK % 2 == 0, "an even number of steps leaves the last in the second set");
-    for (int st = 0; st < ns; ++st) {
-      enter(st);
-#pragma unroll
-      for (int j = 0; j < kK; j += 2) {
-        read(st, j, x0, w0);
-        multiply(x1, w1);
-        interleave();
-        read(st, j + 1, x1, w1);
-        multiply(x0, w0);
-        interleave();
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    multiply(x1, w1);
+    __builtin_amdgcn_sched_barrier(0);
   }
+  multiply(x1, w1);
 #pragma unroll
   for (int i = 0; i < kFm; ++i)
 #pragma unroll
@@ -427,10 +402,11 @@ __global__ __launch_bounds__(256) void few_gemm(GemmArgs a) {
 __device__ __forceinline__ void add_product(v4i& acc, const v4i& w, const v4i& x) {
   asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
 }
-// The products are complete: an accumulator may be read.
-__device__ __forceinline__ void settle(v4i (&acc)[8][8]) {
-  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[7][0]), "+a"(acc[7][1]), "+a"(acc[7][2]), "+a"(acc[7][3]),
-               "+a"(acc[7][4]), "+a"(acc[7][5]), "+a"(acc[7][6]), "+a"(acc[7][7]));
+// The products issued before are complete: their accumulators may be read,
+// moved or written by other instructions. (The compiler does not see what an
+// asm block issues, so it counts no such wait itself.)
+__device__ __forceinline__ void products_done() {
+  asm volatile("s_nop 15\n\ts_nop 7" : : : "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -438,30 +414,30 @@ __device__ __forceinline__ void settle(v4i (&acc)[8][8]) {
 // one wave a SIMD with its 256 accumulators in the accumulation registers and
 // two steps' operands (64 k) in the others. (Eight waves of 128 x 64 read
 // half as much again from LDS, which with the loads' writes was as busy as
-// the matrix units: 472 us for the whole call at the size below, now 435.) A step is eight groups of
-// eight products; the first four read the next step's operands, and each
-// group issues its part of the loads of the stage R - 1 ahead. RB: bytes of k
-// a stage (64 and a ring of five instead of 128 and two: whole lines of the
-// L2 are asked for twice, 480 us against 440).
+// the matrix units: 472 us for the whole call at the size below, now 435.) A
+// step is eight groups of eight products; the first four read the next step's
+// operands, and each group issues its part of the loads of the stage R - 1
+// ahead. (Stages of 64 bytes a row in a ring of five instead of 128 in one of
+// two ask the L2 for its lines twice: 480 us against 440.)
 // Bound by the matrix units at the clock they leave: 4096 x 4096 by 28672 in
 // 430 us, 2.2 P operations a second, products 51% of the cycles at 1.87 GHz
 // (the same product's int32 sums alone take the library 529 us); the rest is
 // the wait for a stage (1.6 us for 1.1 us of products) and, once a tile, the
 // first stage and the store.
-template <typename T, int RB, int R>
+template <typename T, int R>
 __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
+  constexpr int RB = 128;  // bytes of k a stage, two steps
   constexpr int kRows = 1024 / RB, kPer = 512 / kRows / 4;  // rows a load, loads a wave and stage
   constexpr int kK = RB / 64;
   constexpr uint32_t kStage = 512 * RB;
-  static_assert(kPer % 8 == 0 && kPer <= 64 && (kK == 1 || kK == 2), "whole loads a group of products");
+  static_assert(kPer % 8 == 0 && kK == 2, "whole loads a group of products, two steps a stage");
   __shared__ __attribute__((aligned(1024))) char ring[R * kStage];
   const int lane = (int)(threadIdx.x & 63);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r16 = lane & 15, g = lane >> 4;
   const int2 tile = tile_of(a, 1);
   const int tm = tile.x, tn = tile.y;
-  // An even number of steps: x's codes are zero up to a multiple of kPadK.
-  const int ns = (a.k + 127) / 128 * (128 / RB);
+  const int ns = (a.k + RB - 1) / RB;  // (x's codes are zero up to a multiple of kPadK)
 
   // Waves 0 and 1 bring x's rows, 2 and 3 w's; rows past the last repeat it,
   // and w's rows end at their last chunk.
@@ -540,18 +516,13 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
     w0[i] = lds_read_frag<v4i>(woff[0] + i * 16 * RB);
     x0[i] = lds_read_frag<v4i>(xoff[0] + i * 16 * RB);
   }
-  if constexpr (kK == 1) {
-    for (int st = 0; st < ns; st += 2) {
-      step(st + 1, 0, x0, w0, x1, w1);
-      step(st + 2, 0, x1, w1, x0, w0);
-    }
-  } else {
-    for (int st = 0; st < ns; ++st) {
-      step(st, kK - 1, x0, w0, x1, w1);
-      step(st + 1, 0, x1, w1, x0, w0);
-    }
+  for (int st = 0; st < ns; ++st) {
+    step(st, 1, x0, w0, x1, w1);
+    step(st + 1, 0, x1, w1, x0, w0);
+    // Here, not after the loop, where moves of accumulators may come first
+    // (24 cycles in 4,096).
+    products_done();
   }
-  settle(acc);
   li_wait_vm<0>();
   lds_barrier();  // every load is in and every wave has read its last operands: the ring is free
   const int m0 = tm * 256 + wm * 128, n0 = tn * 256 + wn * 128;
@@ -745,7 +716,7 @@ void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
       GemmArgs b = a;
       b.mt = cdiv(a.m, 256);
       b.nt = cdiv(a.n, 256);
-      hipLaunchKernelGGL((wide_gemm<T, 128, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(256), 0, s, b);
+      hipLaunchKernelGGL((wide_gemm<T, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(256), 0, s, b);
       break;
     }
   }
