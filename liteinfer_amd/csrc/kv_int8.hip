@@ -32,7 +32,9 @@
 // launch's other work-groups.
 //
 // Bound by launch and two dependent round trips (slots, then rows and the old
-// scale) at a decode step, by memory in a long pass.
+// scale) at a decode step (4 to 128 tokens, 32 / 8 heads: 6 us), by memory in
+// a long pass (5,569 tokens at head_dim 128: 152 MB in 37.5 us, 4.1 TB/s where
+// a copy moves 4.8).
 #include "li_common.h"
 
 #include <cmath>
