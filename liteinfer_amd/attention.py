@@ -229,11 +229,16 @@ def _paged_packed(query: torch.Tensor, kv: PagedKV, scaling: float, num_kv_group
             out = _paged_decode_step(query.permute(2, 1, 0, 3), kv, scaling, num_kv_groups)  # [T, H, 1, D]
             return out.permute(2, 1, 0, 3)
         one_query_rows = _one_query_rows_to_decode_kernel(kv.host_query_lens)
+    # What an int8 pool's copy has to hold; a captured pass may be replayed
+    # over longer contexts, so its copy has room for all the table names.
+    context_tokens = None
+    if kv.key_scales is not None and kv.host_context_lens and not torch.cuda.is_current_stream_capturing():
+        context_tokens = sum(kv.host_context_lens)
     out = paged_prefill(
         query.squeeze(0).transpose(0, 1), kv.key_pool, kv.value_pool, kv.slot_table, kv.context_lens,
         kv.query_start_loc, kv.max_query_len, scaling, num_kv_groups, one_query_rows=one_query_rows,
         k_scale=kv.k_scale, v_scale=kv.v_scale, key_scales=kv.key_scales, value_scales=kv.value_scales,
-        context_tokens=sum(kv.host_context_lens) if kv.key_scales is not None and kv.host_context_lens else None,
+        context_tokens=context_tokens,
     )
     return out.transpose(0, 1).unsqueeze(0)
 

@@ -227,6 +227,8 @@ def linear_int8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> t
     if flat.stride(-1) != 1:
         flat = flat.contiguous()
     rows = flat.shape[0]
+    if max(rows, n) >= 2 ** 31:
+        raise ValueError(f"linear_int8 takes fewer than 2^31 rows and channels, got {rows} and {n}")
     if not x.is_cuda:
         xc, xs = quantize_rows(flat)
         sums = xc.to(torch.float64) @ codes.to(torch.float64).t()  # whole numbers below 2^31: exact

@@ -411,6 +411,34 @@ def test_a_captured_step_replays_for_other_contexts():
             batch.check(out, half_step(F16))
 
 
+def test_a_captured_packed_pass_replays_for_longer_contexts():
+    """Through the payload, whose host lengths are those of the capture."""
+    batch = Batch(contexts=[300, 90, 40], queries=[100, 20, 1], width=1000)
+    keys, values, ks, vs = batch.store()
+    contexts, starts = batch.contexts_t, torch.from_numpy(batch.starts).to(DEV)
+    query = batch.query.transpose(0, 1).unsqueeze(0)
+    kv = PagedKV(keys, values, batch.table_t, contexts, query_start_loc=starts, max_query_len=100,
+                 host_context_lens=(300, 90, 40), host_query_lens=(100, 20, 1), key_scales=ks, value_scales=vs)
+
+    def call():
+        return paged_attention(query, kv, batch.scaling, batch.groups)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for lens in ([300, 90, 40], [1000, 700, 999], [100, 20, 1], [640, 1000, 3]):
+        batch.contexts = lens
+        contexts.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_packed(batch, out[0].transpose(0, 1))
+
+
 def test_two_calls_on_two_streams():
     batches = [Batch(contexts=[4000, 300, 77], width=6000, seed=s) for s in range(2)]
     stores = [b.store() for b in batches]

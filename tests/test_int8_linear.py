@@ -125,3 +125,9 @@ def test_the_plan_holds_the_rows_codes_and_scales():
     assert lib.li_linear_int8_plan(0, 4096, 4096, ctypes.byref(need)) == _native.LI_OK and need.value == 0
     assert lib.li_linear_int8_plan(1, 4096, 0, ctypes.byref(need)) == _native.LI_EINVAL
     assert lib.li_linear_int8_plan(1, 4096, 131073, ctypes.byref(need)) == _native.LI_EUNSUPPORTED
+
+
+def test_more_rows_than_an_int_counts_are_refused():
+    rows = torch.zeros(1, 16).expand(2 ** 31 + 5, 16)
+    with pytest.raises(ValueError, match="fewer than 2"):
+        ops.linear_int8(rows, torch.zeros(4, 16, dtype=torch.int8), torch.ones(4))
