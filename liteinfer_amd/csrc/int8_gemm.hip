@@ -413,27 +413,30 @@ __device__ __forceinline__ void products_done() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The same for many rows: 256 x 256 outputs of four waves, 128 x 128 each,
-// one wave a SIMD with its 256 accumulators in the accumulation registers and
-// two steps' operands (64 k) in the others. (Eight waves of 128 x 64 read
-// half as much again from LDS, which with the loads' writes was as busy as
-// the matrix units: 472 us for the whole call at the size below, now 435.) A
-// step is eight groups of eight products; the first four read the next step's
-// operands, and each group issues its part of the loads of the stage R - 1
-// ahead. (Stages of 64 bytes a row in a ring of five instead of 128 in one of
-// two ask the L2 for its lines twice: 480 us against 440.)
+// The same for many rows: 256 x 256 outputs of four waves, 128 x 128 each, one
+// wave a SIMD with its 256 accumulators in the accumulation registers and two
+// steps' operands (64 k) in the others; or 256 x 128, 128 x 64 a wave, with a
+// ring of three stages for two. (Eight waves of 128 x 64 read half as much
+// again from LDS, which with the loads' writes was as busy as the matrix
+// units: 472 us for the whole call at the size below, now 435.) A step is FM
+// groups of FN products; the first of them read the next step's operands, and
+// each group issues its part of the loads of the stage R - 1 ahead. (Stages of
+// 64 bytes a row in a ring of five instead of 128 in one of two ask the L2 for
+// its lines twice: 480 us against 440.)
 // Bound by the matrix units at the clock they leave: 4096 x 4096 by 28672 in
 // 430 us, 2.2 P operations a second, products 51% of the cycles at 1.87 GHz
 // (the same product's int32 sums alone take the library 529 us); the rest is
 // the wait for a stage (1.6 us for 1.1 us of products) and, once a tile, the
 // first stage and the store.
-template <typename T, int R>
+template <typename T, int FM, int FN, int R>
 __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
-  constexpr int RB = 128;  // bytes of k a stage, two steps
-  constexpr int kRows = 1024 / RB, kPer = 512 / kRows / 4;  // rows a load, loads a wave and stage
+  constexpr int BM = 32 * FM, BN = 32 * FN;  // 2 x 2 waves of FM x FN groups of 16
+  constexpr int RB = 128;                    // bytes of k a stage, two steps
+  constexpr int kRows = 1024 / RB, kPer = (BM + BN) / kRows / 4;  // rows a load, loads a wave and stage
   constexpr int kK = RB / 64;
-  constexpr uint32_t kStage = 512 * RB;
-  static_assert(kPer % 8 == 0 && kK == 2, "whole loads a group of products, two steps a stage");
+  constexpr int kEach = (kPer + FM - 1) / FM;  // loads with a group of products
+  constexpr uint32_t kStage = (BM + BN) * RB;
+  static_assert(kK == 2 && kEach <= FN && 2 * (FM + FN) <= FM * FN, "two steps a stage; room for its loads and reads");
   __shared__ __attribute__((aligned(1024))) char ring[R * kStage];
   const int lane = (int)(threadIdx.x & 63);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -442,41 +445,43 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
   const int tm = tile.x, tn = tile.y;
   const int ns = (a.k + RB - 1) / RB;  // (x's codes are zero up to a multiple of kPadK)
 
-  // Waves 0 and 1 bring x's rows, 2 and 3 w's; rows past the last repeat it,
-  // and w's rows end at their last chunk.
-  const bool of_x = wv < 2;
-  const int64_t stride = of_x ? a.x_s : a.w_s;
-  const int first = (of_x ? tm : tn) * 256, last = (of_x ? a.m : a.n) - 1;
-  const char* src = (of_x ? a.x : a.w) + first * stride;
-  const int cap = of_x ? 0x7fffffff : (a.k + 15) / 16 * 16 - 16;
+  // A stage's rows, x's first, a quarter to a wave; rows past an operand's
+  // last repeat it, and w's rows end at their last chunk.
+  const char* xsrc = a.x + (int64_t)tm * BM * a.x_s;
+  const char* wsrc = a.w + (int64_t)tn * BN * a.w_s;
+  const int wcap = (a.k + 15) / 16 * 16 - 16;
   uint32_t row_at[kPer];
   int col[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int row = 128 * (wv & 1) + kRows * i + lane / (RB / 16);
-    row_at[i] = (uint32_t)min(row, last - first) * (uint32_t)stride;
+    const int row = kRows * (wv * kPer + i) + lane / (RB / 16);
+    const bool of_x = kRows * (wv * kPer + i) < BM;
+    row_at[i] = of_x ? (uint32_t)min(row, a.m - 1 - tm * BM) * (uint32_t)a.x_s
+                     : (uint32_t)min(row - BM, a.n - 1 - tn * BN) * (uint32_t)a.w_s;
     col[i] = 16 * ((lane % (RB / 16)) ^ swizzle<RB>(row));
   }
   const uint32_t base = lds_addr(&ring[0]);
-  const uint32_t mine = base + (uint32_t)wv * 128 * RB;
+  const uint32_t mine = base + (uint32_t)wv * kPer * 1024;
   auto load = [&](int st, uint32_t to, int i) __attribute__((always_inline)) {
-    dma16_at(src, row_at[i] + (uint32_t)min(col[i] + st * RB, cap), mine + to + 1024 * i);
+    const bool of_x = kRows * (wv * kPer + i) < BM;
+    const int at = col[i] + st * RB;
+    dma16_at(of_x ? xsrc : wsrc, row_at[i] + (uint32_t)min(at, of_x ? 0x7fffffff : wcap), mine + to + 1024 * i);
   };
 
-  v4i acc[8][8];
+  v4i acc[FM][FN];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    for (int j = 0; j < FN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
   const int wm = wv & 1, wn = wv >> 1;
   uint32_t xoff[kK], woff[kK];
 #pragma unroll
   for (int j = 0; j < kK; ++j) {
     const uint32_t o = base + (uint32_t)(r16 * RB + 16 * ((4 * j + g) ^ swizzle<RB>(r16)));
-    xoff[j] = o + (uint32_t)wm * 128 * RB;
-    woff[j] = o + (uint32_t)(256 + wn * 128) * RB;
+    xoff[j] = o + (uint32_t)wm * (BM / 2) * RB;
+    woff[j] = o + (uint32_t)(BM + wn * (BN / 2)) * RB;
   }
-  v4i x0[8], x1[8], w0[8], w1[8];
+  v4i x0[FM], x1[FM], w0[FN], w1[FN];
   uint32_t here = 0, fill = (R - 1) * kStage;  // the ring's stage that is read from, and the one to load into
   // Stage st is here (all of it, once every wave has come), and the one before it is free.
   auto enter = [&]() __attribute__((always_inline)) {
@@ -489,19 +494,19 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
   // the same stage, or of stage `st`, entered first. (Past the last stage the
   // last is loaded once more and what is read is not used: without branches
   // the accumulators stay where they are.)
-  auto step = [&](int st, int j, const v4i (&xa)[8], const v4i (&wa)[8], v4i (&xb)[8], v4i (&wb)[8])
+  auto step = [&](int st, int j, const v4i (&xa)[FM], const v4i (&wa)[FN], v4i (&xb)[FM], v4i (&wb)[FN])
       __attribute__((always_inline)) {
     const bool entered = j == 0;
     if (entered) enter();
     const int ahead = min(st + R - 1, ns - 1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < FM; ++i) {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        if (entered && f < kPer / 8) load(ahead, fill, i * (kPer / 8) + f);
-        const int r = (8 * i + f) / 2;
-        if (f % 2 == 0 && r < 8) wb[r] = lds_read_frag<v4i>(woff[j] + here + r * 16 * RB);
-        else if (f % 2 == 0 && r < 16) xb[r - 8] = lds_read_frag<v4i>(xoff[j] + here + (r - 8) * 16 * RB);
+      for (int f = 0; f < FN; ++f) {
+        if (entered && f < kEach && i * kEach + f < kPer) load(ahead, fill, i * kEach + f);
+        const int r = (FN * i + f) / 2;
+        if (f % 2 == 0 && r < FN) wb[r] = lds_read_frag<v4i>(woff[j] + here + r * 16 * RB);
+        else if (f % 2 == 0 && r < FN + FM) xb[r - FN] = lds_read_frag<v4i>(xoff[j] + here + (r - FN) * 16 * RB);
         add_product(acc[i][f], wa[f], xa[i]);
         if (f % 2) __builtin_amdgcn_sched_barrier(0);
       }
@@ -515,56 +520,56 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
   li_wait_vm<(R - 1) * kPer>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w0[i] = lds_read_frag<v4i>(woff[0] + i * 16 * RB);
-    x0[i] = lds_read_frag<v4i>(xoff[0] + i * 16 * RB);
-  }
+  for (int i = 0; i < FN; ++i) w0[i] = lds_read_frag<v4i>(woff[0] + i * 16 * RB);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) x0[i] = lds_read_frag<v4i>(xoff[0] + i * 16 * RB);
   for (int st = 0; st < ns; ++st) {
     step(st, 1, x0, w0, x1, w1);
     step(st + 1, 0, x1, w1, x0, w0);
     // Here, not after the loop, where moves of accumulators may come first
-    // (24 cycles in 4,096).
+    // (24 cycles in 4,096 of the largest tile).
     products_done();
   }
   li_wait_vm<0>();
   lds_barrier();  // every load is in and every wave has read its last operands: the ring is free
-  const int m0 = tm * 256 + wm * 128, n0 = tn * 256 + wn * 128;
+  const int m0 = tm * BM + wm * (BM / 2), n0 = tn * BN + wn * (BN / 2);
   if constexpr (sizeof(T) == 2) {
-    if (a.rows16 && n0 + 128 <= a.n) {
+    if (a.rows16 && n0 + BN / 2 <= a.n) {
       // A lane holds four neighbours of a row, 16 rows to an instruction: stored
       // as they are every store would write 32-byte pieces (the stores alone
-      // took a quarter of the call). Each wave turns its 128 rows of 256 bytes
-      // in its own part of the ring instead, chunk c of row r at c ^ r % 16, and
-      // stores whole rows.
-      static_assert(R * kStage >= 4 * 128 * 256, "the ring holds the waves' rows");
-      const uint32_t rows = base + (uint32_t)wv * (128 * 256);
-      floatx4_t ws[8];
+      // took a quarter of the call). Each wave turns its rows in its own part
+      // of the ring instead, chunk c of row r at c ^ r % kCh, and stores whole
+      // rows.
+      constexpr int kRowBytes = BN, kCh = kRowBytes / 16, kRowsEach = 64 / kCh;
+      static_assert(R * kStage >= 4 * (BM / 2) * kRowBytes, "the ring holds the waves' rows");
+      const uint32_t rows = base + (uint32_t)wv * (BM / 2 * kRowBytes);
+      floatx4_t ws[FN];
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < FN; ++f) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) ws[f][r] = a.ws[n0 + 16 * f + 4 * g + r];
       }
       typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < FM; ++i) {
         const int row = 16 * i + r16;
         const float sx = a.xs[min(m0 + row, a.m - 1)];
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
+        for (int f = 0; f < FN; ++f) {
           float v[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = (float)acc[i][f][r] * sx * ws[f][r];
           const int c = 2 * f + (g >> 1);
           *reinterpret_cast<__attribute__((address_space(3))) u32x2_t*>(
-              (uintptr_t)(rows + row * 256 + 16 * (c ^ r16) + 8 * (g & 1))) =
+              (uintptr_t)(rows + row * kRowBytes + 16 * (c ^ (row % kCh)) + 8 * (g & 1))) =
               u32x2_t{li_pack2<T>(v[0], v[1]), li_pack2<T>(v[2], v[3])};
         }
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int row = 4 * i + g, c = r16;
-        const u32x4_t v = lds_read_frag<u32x4_t>(rows + row * 256 + 16 * (c ^ (row & 15)));
+      for (int i = 0; i < BM / 2 / kRowsEach; ++i) {
+        const int row = kRowsEach * i + lane / kCh, c = lane % kCh;
+        const u32x4_t v = lds_read_frag<u32x4_t>(rows + row * kRowBytes + 16 * (c ^ (row % kCh)));
         if (m0 + row < a.m)
           __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(a.out + ((int64_t)(m0 + row) * a.o_s + n0 + 8 * c) * 2));
       }
@@ -572,9 +577,9 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int f = 0; f < 8; ++f) {
+    for (int f = 0; f < FN; ++f) {
       store4<T>(a, acc[i][f], 0, m0 + 16 * i + r16, n0 + 16 * f + 4 * g);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -611,7 +616,7 @@ constexpr int kFewLeft = 64;
 constexpr int64_t kWideStride = int64_t(1) << 23;  // 255 rows of it and a row's bytes stay below 2^32
 
 // Which kernel a product runs on and the runs its k is cut into.
-enum Kind { kFew, kSome, kMany, kMost };
+enum Kind { kFew, kSome, kMany, kHalf, kMost };
 struct Plan {
   Kind kind;
   int bm, bn, splits;
@@ -620,23 +625,26 @@ struct Plan {
 // 16 us for 20 at 100 x 4096 by 4096, 17 for 22 at 256 rows, 12 for 18 at 300 x
 // 2048 by 2048; with more of them than compute units 128 x 128 wins (52 for 40
 // at 100 x 4096 by 28672).
-// Above, a round of tiles of 256 x 256 (one a compute unit) takes as long as
-// 2.2 rounds of 128 x 128 for four times the work, so what the last round
-// leaves idle decides. Against 128 x 128: 71 us for 120 at 512 x 4096 by 28672
-// (1 round, 4), 76 for 88 at 1300 x 4096 by 6144 (1, 3), 119 for 145 at 3000
-// (2, 5), 255 for 412 at 2048 by 28672; but 85 for 67 at 2048 x 4096 by 4096
-// (1, 2), 80 for 62 at 1000 x 4096 by 6144 (1, 2).
+// Above, the last round of tiles (one a compute unit) decides, by what it
+// leaves idle: a round of 128 x 128, 256 x 128 and 256 x 256 takes about 30, 37
+// and 62 us at k = 4096. 256 x 128 against 128 x 128: 46 us for 69 at 256 x 4096
+// by 28672 (1 round, 2), 43 for 63 at 1000 by 6144 and 46 for 67 at 2048 by 4096
+// (1, 2), but 113 for 89 at 1000 x 14336 by 4096 (1, 1). 256 x 256 against 256 x
+// 128: 72 for 77 at 512 by 28672 and 69 for 77 at 2000 by 6144 (1, 2), but 126
+// for 115 at 600 by 28672 (2, 3) and 67 for 43 at 1000 by 6144 (1, 1).
 // Tiles that leave a quarter of the GPU idle cut k, to runs of 1,024 at least:
 // 40 us -> 24 at 64 x 14336 by 4096, 77 -> 28 at 100 rows.
 Plan plan_of(int m, int n, int k) {
   const int cus = li::device_cu_count();
   const auto rounds = [&](int64_t tm, int64_t tn) { return (tm * tn + cus - 1) / cus; };
-  const int left = m % 256;
-  const int64_t large = rounds(left && left <= kFewLeft ? m / 256 : cdiv(m, 256), cdiv(n, 256));
+  const int left = m % 256, tall = left && left <= kFewLeft && m > left ? m / 256 : cdiv(m, 256);
+  const int64_t many = 5 * rounds(cdiv(m, 128), cdiv(n, 128)), half = 6 * rounds(tall, cdiv(n, 128));
+  const int64_t most = 10 * rounds(tall, cdiv(n, 256));
   Plan p{};
   if (m <= 16) p = {kFew, 16, 16, 1};
   else if (m <= 64 || (int64_t)cdiv(m, 64) * cdiv(n, 64) <= cus) p = {kSome, 64, 64, 1};
-  else if (4 * rounds(cdiv(m, 128), cdiv(n, 128)) <= 9 * large) p = {kMany, 128, 128, 1};
+  else if (many <= std::min(half, most)) p = {kMany, 128, 128, 1};
+  else if (half <= most) p = {kHalf, 256, 128, 1};
   else p = {kMost, 256, 256, 1};
   const int64_t tiles = (int64_t)cdiv(m, p.bm) * cdiv(n, p.bn);
   if ((p.kind == kSome || p.kind == kMany) && tiles * 4 < cus * 3)
@@ -694,13 +702,20 @@ void launch_ring(GemmArgs a, hipStream_t s) {
   hipLaunchKernelGGL((ring_gemm<T, BM, BN, WM, WN, RB, R>), grid, block, 0, s, a);
 }
 
+template <typename T, int FM, int FN, int R>
+void launch_wide(GemmArgs a, hipStream_t s) {
+  a.mt = cdiv(a.m, 32 * FM);
+  a.nt = cdiv(a.n, 32 * FN);
+  hipLaunchKernelGGL((wide_gemm<T, FM, FN, R>), dim3((unsigned)(a.mt * a.nt)), dim3(256), 0, s, a);
+}
+
 template <typename T>
 void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
   const int left = a.m % 256;
-  if (kind == kMost && left && left <= kFewLeft) {
+  if (kind >= kHalf && left && left <= kFewLeft && a.m > left) {
     GemmArgs whole = a, rest = a;
     whole.m = a.m - left;
-    launch_gemm<T>(whole, kMost, s);
+    launch_gemm<T>(whole, kind, s);
     rest.x += (int64_t)whole.m * a.x_s;
     rest.xs += whole.m;
     rest.out += (int64_t)whole.m * a.o_s * (int64_t)sizeof(T);
@@ -715,13 +730,8 @@ void launch_gemm(const GemmArgs& a, Kind kind, hipStream_t s) {
       break;
     case kSome: launch_ring<T, 64, 64, 2, 2, 256, 4>(a, s); break;
     case kMany: launch_ring<T, 128, 128, 2, 2, 128, 4>(a, s); break;
-    case kMost: {
-      GemmArgs b = a;
-      b.mt = cdiv(a.m, 256);
-      b.nt = cdiv(a.n, 256);
-      hipLaunchKernelGGL((wide_gemm<T, 2>), dim3((unsigned)(b.mt * b.nt)), dim3(256), 0, s, b);
-      break;
-    }
+    case kHalf: launch_wide<T, 8, 4, 3>(a, s); break;
+    case kMost: launch_wide<T, 8, 8, 2>(a, s); break;
   }
   if (a.splits > 1) {
     const int64_t work = (int64_t)a.m * ((a.n + 3) / 4);
@@ -796,7 +806,7 @@ extern "C" int li_linear_int8(const void* x, int64_t x_stride, const void* w, in
   a.rows16 = out_stride % 8 == 0 && li::aligned16(out);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // (The large tiles reach their rows by 32-bit offsets.)
-  const Kind kind = p.kind == kMost && w_stride > kWideStride ? kMany : p.kind;
+  const Kind kind = p.kind >= kHalf && w_stride > kWideStride ? kMany : p.kind;
   if (dtype == LI_F32) launch_gemm<float>(a, kind, s);
   else if (dtype == LI_F16) launch_gemm<li_f16>(a, kind, s);
   else launch_gemm<li_bf16>(a, kind, s);

@@ -58,9 +58,10 @@ def test_sizes_of_the_engine(shape, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("shape", [(530, 2051, 77), (530, 2051, 2100), (1300, 6147, 131), (1400, 6147, 131), (1283, 6148, 300),
-                                   (1290, 6152, 128)])
+                                   (1290, 6152, 128), (2000, 6147, 131), (2064, 6147, 131), (2051, 6152, 128), (200, 28685, 131),
+                                   (68, 40000, 64), (320, 20001, 16)])
 def test_large_tiles_at_odd_sizes(shape, dtype):
-    """128 x 128 whole and cut along k; 256 x 256 with 20, 120, 3 and 10 rows past the last whole one."""
+    """128 x 128 whole and cut along k, 256 x 128 and 256 x 256, with few and with many rows past the last whole tile."""
     x, codes, scales = _operands(*shape, dtype)
     _check(ops.linear_int8(x.to(DEV), *_weight(codes, scales)), x, codes, scales)
 
