@@ -450,8 +450,9 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
   const char* xsrc = a.x + (int64_t)tm * BM * a.x_s;
   const char* wsrc = a.w + (int64_t)tn * BN * a.w_s;
   const int wcap = (a.k + 15) / 16 * 16 - 16;
+  const char* src[kPer];
   uint32_t row_at[kPer];
-  int col[kPer];
+  int col[kPer], cap[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int row = kRows * (wv * kPer + i) + lane / (RB / 16);
@@ -459,13 +460,13 @@ __global__ __launch_bounds__(256, 1) void wide_gemm(GemmArgs a) {
     row_at[i] = of_x ? (uint32_t)min(row, a.m - 1 - tm * BM) * (uint32_t)a.x_s
                      : (uint32_t)min(row - BM, a.n - 1 - tn * BN) * (uint32_t)a.w_s;
     col[i] = 16 * ((lane % (RB / 16)) ^ swizzle<RB>(row));
+    src[i] = of_x ? xsrc : wsrc;
+    cap[i] = of_x ? 0x7fffffff : wcap;
   }
   const uint32_t base = lds_addr(&ring[0]);
   const uint32_t mine = base + (uint32_t)wv * kPer * 1024;
   auto load = [&](int st, uint32_t to, int i) __attribute__((always_inline)) {
-    const bool of_x = kRows * (wv * kPer + i) < BM;
-    const int at = col[i] + st * RB;
-    dma16_at(of_x ? xsrc : wsrc, row_at[i] + (uint32_t)min(at, of_x ? 0x7fffffff : wcap), mine + to + 1024 * i);
+    dma16_at(src[i], row_at[i] + (uint32_t)min(col[i] + st * RB, cap[i]), mine + to + 1024 * i);
   };
 
   v4i acc[FM][FN];
