@@ -18,6 +18,11 @@
 // The query and the output are multiplied by the same powers. Each division
 // is exact (scales are multiplied by the inverse), each value rounded once.
 //
+// Where V's scale is not finite, the row of K is laid out as NaN and V's as
+// zeros: who reads the key gets a NaN weight, and so the NaN in every dim that
+// V would give, while a query in front of it, for whom the key is masked, does
+// not multiply its weight of zero by a NaN.
+//
 // Two launches, both bound by memory and its latency. largest_scales:
 // work-groups take kThreads positions of a sequence each (kParts of them at
 // most) and keep the largest scale of each head of the blocks they lie in.
@@ -82,6 +87,12 @@ __device__ __forceinline__ void widen(const u32x4_t x, float scale, li_f16* dst)
   }
   reinterpret_cast<u32x4_t*>(dst)[0] = out[0];
   reinterpret_cast<u32x4_t*>(dst)[1] = out[1];
+}
+
+__device__ __forceinline__ void fill(uint32_t two, li_f16* dst) {
+  const u32x4_t x = {two, two, two, two};
+  reinterpret_cast<u32x4_t*>(dst)[0] = x;
+  reinterpret_cast<u32x4_t*>(dst)[1] = x;
 }
 
 // The exponent e (biased) of a scale s < 2^(e + 1), held where every power
@@ -212,8 +223,15 @@ __global__ __launch_bounds__(kThreads) void copy_contexts(CopyArgs a) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         if (dst[u] < 0) continue;
-        widen(k[u], ks[u] * inverse_unit(top[head[u]], false), static_cast<li_f16*>(a.keys) + dst[u]);
-        widen(v[u], vs[u] * inverse_unit(top[a.num_kv_heads + head[u]], true), static_cast<li_f16*>(a.values) + dst[u]);
+        li_f16* kd = static_cast<li_f16*>(a.keys) + dst[u];
+        li_f16* vd = static_cast<li_f16*>(a.values) + dst[u];
+        if ((__float_as_uint(vs[u]) & 0x7fffffffu) < kInfBits) {
+          widen(k[u], ks[u] * inverse_unit(top[head[u]], false), kd);
+          widen(v[u], vs[u] * inverse_unit(top[a.num_kv_heads + head[u]], true), vd);
+        } else {
+          fill(0x7e007e00u, kd);
+          fill(0u, vd);
+        }
       }
     }
   }

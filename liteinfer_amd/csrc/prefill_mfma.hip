@@ -759,10 +759,17 @@ struct PpLds {
 
 
 // LDS of a ping-pong work-group; prefill_pp_rows's row waves use it first.
-// x rounded to fp16 stays finite where x is.
-__device__ __forceinline__ float held_to_f16(float x) {
-  const bool finite = (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u;
-  return finite ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+// Two 16-bit values (T's bits, low first) times `unit`, as fp16: finite where
+// they are, NaN where they are not (an infinity in a query gives NaN scores
+// either way). Told apart as integers: the compiler takes floats for numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t times_to_f16(uint32_t two, float unit) {
+  constexpr uint32_t kInf = std::is_same_v<T, li_f16> ? 0x7c00u : 0x7f80u;
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const t2 x = __builtin_bit_cast(t2, two);
+  auto held = [](float v) { return fminf(fmaxf(v, -65504.f), 65504.f); };
+  const uint32_t y = li_pack2<li_f16>(held((float)x[0] * unit), held((float)x[1] * unit));
+  return ((two & 0x7fffu) >= kInf ? 0x7e00u : y & 0xffffu) | ((two >> 16 & 0x7fffu) >= kInf ? 0x7e000000u : y & 0xffff0000u);
 }
 
 template <int D, int KVR>
@@ -919,7 +926,7 @@ __device__ __forceinline__ void prefill_pp_body(AttnArgs a, const AttnArgs& d) {
         u32x4_t pw;
 #pragma unroll
         for (int u2 = 0; u2 < 4; ++u2) {
-          if constexpr (kCopied) pw[u2] = li_pack2<T>(held_to_f16((float)x[2 * u2] * k_unit), held_to_f16((float)x[2 * u2 + 1] * k_unit));
+          if constexpr (kCopied) pw[u2] = times_to_f16<TO>(__builtin_bit_cast(u32x4_t, x)[u2], k_unit);
           else pw[u2] = li_pack2<T>((float)x[2 * u2] * sc, (float)x[2 * u2 + 1] * sc);
         }
         qf[nb][j] = __builtin_bit_cast(Frag, pw);

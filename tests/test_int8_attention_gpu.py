@@ -270,6 +270,23 @@ def test_a_block_that_holds_nan_gives_nan_to_its_readers_only():
             assert not nan.any()
 
 
+@pytest.mark.parametrize("of", [0, 1], ids=["keys", "values"])
+@pytest.mark.parametrize("dim", [128, 64, 80])
+@pytest.mark.parametrize("context, queries", [(70, 30), (2100, 300), (900, 900)])
+def test_a_token_that_is_not_finite_is_not_seen_before_it(context, queries, dim, of):
+    """Causal: a chunk's queries in front of the NaN do not read it, though it lies in their tile."""
+    batch = Batch(contexts=[context, 40], queries=[queries, 1], dim=dim, width=3000)
+    batch.table %= 32 * 16
+    at = context - 10
+    batch.table[0, at] = 50 * 16 + 2
+    batch.scales[of][50, 0] = np.nan
+    nan = torch.isnan(batch.prefill())
+    first = queries - 10
+    assert nan[first:queries, :batch.groups].all()
+    nan[first:queries, :batch.groups] = False
+    assert not nan.any()
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_a_query_that_is_not_finite_gives_nan(value):
     for width in (0, 4000):
@@ -280,6 +297,26 @@ def test_a_query_that_is_not_finite_gives_nan(value):
         nan = torch.isnan(out)
         nan[1, 2] = False
         assert not nan.any()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dim", [128, 64])
+def test_a_chunks_query_that_is_not_finite_gives_nan(dim, value):
+    for context in (70, 2100):
+        batch = Batch(contexts=[context, 40], queries=[60, 1], dim=dim, width=3000)
+        batch.query[17, 2, 5] = value
+        nan = torch.isnan(batch.prefill())
+        assert nan[17, 2].all()
+        nan[17, 2] = False
+        assert not nan.any()
+
+
+def test_sequences_without_queries_beside_chunks():
+    """Nothing is laid out for them, whatever they hold."""
+    batch = Batch(contexts=[300, 500, 90, 0, 40], queries=[100, 0, 20, 0, 1], width=1000)
+    _check_packed(batch, batch.prefill())
+    tokens = batch.prefill(context_tokens=930)
+    _check_packed(batch, tokens)
 
 
 def test_queries_of_very_different_sizes():
